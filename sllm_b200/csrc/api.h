@@ -91,6 +91,16 @@ int sllm_prefill_attention(const void* qkv, int total_tokens, int qkv_ld, const 
                            int hkv, int hd, int window, float sm_scale, const float* sinks, void* out_bf16,
                            void* out_fp8, float* out_scale, int ld_scale, int* status, void* stream);
 
+/* logprobs.cu */
+int sllm_token_logprobs(const void* logits, long long ld, int rows, int vocab, int dtype, const void* tokens,
+                        int tokens64, int given, int top, float* logprob, float* entropy, int* top_ids,
+                        float* top_logprobs, void* stream);
+
+/* batch_plan.cu */
+int sllm_batch_plan(const int* new_lens, const int* starts, const int* pages, long long page_count, int requests,
+                    int rows, int max_blocks, long long ld_table, int page, int* row_off, int* positions,
+                    int* seq_index, int* kv_lens, long long* slots, long long* last_rows, int* table, void* stream);
+
 /* comm.cu */
 int sllm_symm_alloc(long long bytes, void** dev_ptr, unsigned char* handle64);
 int sllm_symm_open(const unsigned char* handle64, void** dev_ptr);

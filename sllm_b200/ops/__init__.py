@@ -2,6 +2,8 @@
 from .core import (Again, KVLayer, LinearWeight, QTensor, Workspace, add_group_norm, argmax, device_status, elementwise,
                    embed_group_norm, embedding, gated_act, gemm_raw, group_norm, linear, paged_attention, poly_norm, quant_fp8, rmsnorm, rope_kv_append, workspace)
 from ._lib import KernelError, kernels_available
+from .logprobs import TokenLogprobs, linear_logprobs, token_logprobs
+from .plan import BatchPlan, batch_plan
 
 
 def attention(q, kv, batch, hq, hkv, hd, *, window=0, quant_out=False, sm_scale=None, sinks=None, qkv=None):

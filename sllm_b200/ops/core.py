@@ -11,6 +11,7 @@ CausalAttention, AttentionPreprocess (rope_kv_append), Argmax, TokenSelect (ops.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import math
 from dataclasses import dataclass
@@ -118,6 +119,13 @@ def _stream() -> C.c_void_p:
     if _lib.fake_active():
         return C.c_void_p(0)
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def _on(device: torch.device):
+    """Context in which launches go to ``device`` and its current stream."""
+    if device.type != "cuda" or device.index in (None, torch.cuda.current_device()):
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 _SM_COUNT = 148

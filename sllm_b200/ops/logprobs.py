@@ -1,0 +1,137 @@
+"""Log-probabilities of given tokens with the entropy of their rows and the likeliest alternatives: from logits
+(csrc/logprobs.cu) and from hidden rows and the output matrix.  CPU tensors run the restatement below, in 64 bits."""
+from __future__ import annotations
+
+import ctypes as C
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _lib
+
+P, I, L = C.c_void_p, C.c_int, C.c_longlong
+_SIGS = {
+    "sllm_token_logprobs": (I, [P, L, I, I, I, P, I, I, I, P, P, P, P, P]),
+}
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+MAX_TOP = 32
+CHUNK_LOGITS = 1 << 26         # logits that `linear_logprobs` holds at a time where it writes them
+
+
+def _k():
+    for n, s in _SIGS.items():
+        _lib.EXTRA_KERNEL_SIGNATURES.setdefault(n, s)
+    return _lib.kernels()
+
+
+class TokenLogprobs(NamedTuple):
+    """fp32, in nats.  ``top_ids`` / ``top_logprobs`` [R, top]: the largest logits, equal ones by id; -1 / -inf where a row has fewer
+    tokens."""
+    logprob: torch.Tensor                          # of the given tokens, in their shape
+    entropy: torch.Tensor                          # [R]
+    top_ids: Optional[torch.Tensor] = None         # int32
+    top_logprobs: Optional[torch.Tensor] = None
+
+
+def _check_tokens(tokens: torch.Tensor, rows: int, device) -> None:
+    if tokens.dtype not in (torch.int32, torch.int64) or tokens.dim() not in (1, 2) or tokens.shape[0] != rows or tokens.device != device:
+        raise ValueError("tokens are int32 or int64 [rows] or [rows, n] on the device of the rows")
+
+
+def _cpu(logits: torch.Tensor, tokens: torch.Tensor, top: int) -> TokenLogprobs:
+    z = logits.double()
+    r, v = z.shape
+    inf = float("inf")
+    nan = torch.isnan(z).any(1)
+    up = (z == inf).any(1)
+    z = torch.where(up[:, None], torch.where(z == inf, torch.zeros_like(z), torch.full_like(z, -inf)), z)
+    empty = (z == -inf).all(1)
+    d = z - z.max(1, keepdim=True).values                  # (first: the logarithm is lost next to a logit of the type's lowest value)
+    logp = torch.where(empty[:, None], z, d - torch.logsumexp(d, 1, keepdim=True))
+    p = torch.exp(logp)
+    entropy = -torch.where(p > 0, p * logp, torch.zeros_like(p)).sum(1)
+    logp = torch.where(nan[:, None], torch.full_like(logp, float("nan")), logp)
+    entropy = torch.where(nan, torch.full_like(entropy, float("nan")), entropy)
+    ids = tokens.long() if tokens.dim() == 2 else tokens.long()[:, None]
+    lp = logp.gather(1, ids.clamp(0, v - 1))
+    lp = torch.where(ids < 0, torch.zeros_like(lp), torch.where(ids >= v, torch.full_like(lp, float("nan")), lp))
+    out = [lp.float().reshape(tokens.shape), entropy.float(), None, None]
+    if top:
+        n = min(top, v)
+        val, at = torch.sort(torch.nan_to_num(logits.double(), nan=-inf, posinf=inf, neginf=-inf), dim=1, descending=True, stable=True)
+        none = (val[:, :n] == -inf) | nan[:, None]
+        top_ids = torch.full((r, top), -1, dtype=torch.int32)
+        top_lp = torch.full((r, top), -inf)
+        top_ids[:, :n] = torch.where(none, -1, at[:, :n]).to(torch.int32)
+        top_lp[:, :n] = torch.where(none, torch.tensor(-inf, dtype=torch.float64), logp.gather(1, at[:, :n])).float()
+        top_lp[nan] = float("nan")
+        out[2:] = [top_ids, top_lp]
+    return TokenLogprobs(*out)
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> TokenLogprobs:
+    """Log-probabilities of ``tokens`` (int32 / int64 [R] or [R, n]) under the rows of ``logits`` (bf16, fp16 or fp32 [R, V], rows of
+    any stride), the rows' entropies and their ``top`` (0 to 32) likeliest tokens.  -inf logits are shut out: a row of nothing else has
+    log-probabilities of -inf, entropy 0 and no alternatives.  A row with +inf is uniform over those; one with NaN gives NaN and no
+    alternatives.  A token below 0 stands for none (0, so that padded places drop out of sums), one from V on gives NaN."""
+    if logits.dim() != 2 or logits.dtype not in _DTYPES or logits.shape[1] < 1 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError("logits are bf16, fp16 or fp32 [rows, vocabulary] with contiguous rows")
+    if not 0 <= top <= MAX_TOP:
+        raise ValueError(f"top lies between 0 and {MAX_TOP}")
+    _check_tokens(tokens, logits.shape[0], logits.device)
+    if _lib.on_cpu(logits):
+        return _cpu(logits, tokens, top)
+    from .core import _on, _p, _stream
+    r, v = logits.shape
+    dev = logits.device
+    tokens = tokens.contiguous()
+    lp = torch.empty(tokens.shape, dtype=torch.float32, device=dev)
+    entropy = torch.empty(r, dtype=torch.float32, device=dev)
+    ids = torch.empty((r, top), dtype=torch.int32, device=dev) if top else None
+    tlp = torch.empty((r, top), dtype=torch.float32, device=dev) if top else None
+    if r:
+        with _on(dev):
+            rc = _k().sllm_token_logprobs(_p(logits), logits.stride(0), r, v, _DTYPES[logits.dtype], _p(tokens), int(tokens.dtype == torch.int64),
+                                          tokens.shape[1] if tokens.dim() == 2 else 1, top, _p(lp), _p(entropy), _p(ids), _p(tlp), _stream())
+        _lib.check(rc, "token_logprobs")
+        if _lib.audit_enabled():
+            _lib.record_dispatch("token_logprobs", "logprobs_kernel", rows=r, vocab=v, top=top)
+    return TokenLogprobs(lp, entropy, ids, tlp)
+
+
+def linear_logprobs(x, w, tokens: torch.Tensor, softcap: float = 0.0, top: int = 0) -> TokenLogprobs:
+    """`token_logprobs` of the logits x W^T (``softcap`` > 0: softcap * tanh(logit / softcap)) for one token per row, in memory that
+    does not grow with rows * vocabulary.  ``x``: hidden rows [R, d] as `ops.linear` takes them for ``w``; ``tokens`` [R].  Logits of
+    dense weights are not rounded on the way (those of FP8 and 4-bit weights are bf16)."""
+    from . import core
+    xd = x.data if isinstance(x, core.QTensor) else x
+    if xd.dim() != 2 or xd.shape[1] != w.in_features:
+        raise ValueError("x is [rows, in_features]")
+    if not 0.0 <= softcap < float("inf"):
+        raise ValueError("the soft cap is finite and positive, or 0 for none")
+    if not 0 <= top <= MAX_TOP:
+        raise ValueError(f"top lies between 0 and {MAX_TOP}")
+    _check_tokens(tokens, xd.shape[0], xd.device)
+    if tokens.dim() != 1:
+        raise ValueError("one token per row")
+    step = max(1, CHUNK_LOGITS // w.out_features)
+    parts = []
+    for lo in range(0, xd.shape[0], step):
+        hi = min(lo + step, xd.shape[0])
+        if isinstance(x, core.QTensor):
+            rows = core.QTensor(x.data[lo:hi], x.scale[:, lo:hi].contiguous())
+        else:
+            rows = x[lo:hi]
+        if w.kind == "dense":
+            z = core.linear(rows, w, act="softcap" if softcap else None, act_arg=softcap, out_fp32=True)
+        else:
+            z = core.linear(rows, w)
+            if softcap:
+                z = core.elementwise("tanh_softcap", z, s=softcap)
+        parts.append(token_logprobs(z, tokens[lo:hi], top))
+    if not parts:
+        z = torch.empty((0, w.out_features), dtype=torch.float32, device=xd.device)
+        return token_logprobs(z, tokens, top)
+    if len(parts) == 1:
+        return parts[0]
+    return TokenLogprobs(*(None if f[0] is None else torch.cat(f) for f in zip(*parts)))

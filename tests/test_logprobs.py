@@ -1,0 +1,290 @@
+"""Log-probabilities of given tokens, entropies and alternatives against the definition in 64 bits."""
+import math
+
+import pytest
+import torch
+
+from sllm_b200 import ops
+from sllm_b200.ops import _lib, logprobs as LP
+
+DEV = "cuda"
+INF, NAN = float("inf"), float("nan")
+EPS = 2.0 ** -24
+
+
+def oracle(z, ids, top):
+    """Row by row from p = exp(z) / sum exp(z), in 64 bits."""
+    lps, hs, tids, tlps = [], [], [], []
+    for row, given in zip(z.double().cpu(), (ids if ids.dim() == 2 else ids[:, None]).tolist()):
+        v = row.numel()
+        if torch.isnan(row).any():
+            logp, h = torch.full((v,), NAN, dtype=torch.float64), NAN
+        elif (row == INF).any():
+            n = int((row == INF).sum())
+            logp, h = torch.where(row == INF, -math.log(n), -INF).double(), math.log(n)
+        elif (row == -INF).all():
+            logp, h = row, 0.0
+        else:
+            w = torch.exp(row - row.max())
+            p = w / w.sum()
+            logp = (row - row.max()) - torch.log(w.sum())
+            h = -float((p[p > 0] * logp[p > 0]).sum())
+        lps.append([0.0 if t < 0 else NAN if t >= v else float(logp[t]) for t in given])
+        hs.append(h)
+        order = [] if math.isnan(h) else [i for i in sorted(range(v), key=lambda i: (-float(row[i]), i))[:top] if row[i] != -INF]
+        tids.append(order + [-1] * (top - len(order)))
+        tlps.append([float(logp[i]) for i in order] + [NAN if math.isnan(h) else -INF] * (top - len(order)))
+    t = lambda x: torch.tensor(x, dtype=torch.float64)
+    return t(lps).reshape(ids.shape), t(hs), torch.tensor(tids).reshape(z.shape[0], top), t(tlps).reshape(z.shape[0], top)
+
+
+def same(got, want, tol):
+    got = got.double().cpu()
+    want = torch.where(want.abs() > torch.finfo(torch.float32).max, torch.sign(want) * INF, want)      # beyond fp32's range
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(torch.isinf(got), torch.isinf(want)) and torch.equal(got[torch.isinf(got)], want[torch.isinf(want)])
+    ok = torch.isfinite(want)
+    err = (got - want).abs()[ok]
+    limit = (torch.as_tensor(tol, dtype=torch.float64).expand(want.shape))[ok]
+    assert bool((err <= limit).all()), f"off by {float((err - limit).max()):.3g} beyond the limit"
+
+
+def check(z, ids, top, got):
+    """Sums of V terms: a chain of at most V / 256 additions per thread and 16 more to join them, each off by 2^-24; an exponential by
+    2^-22; differences and the result by 2^-24 of their size.  The entropy's second sum has the same relative error for each term, the
+    terms having one sign."""
+    lp, h, tid, tlp = oracle(z, ids, top)
+    rel = (z.shape[1] / 256 + 32) * EPS
+    same(got.logprob, lp, rel + 4 * EPS * torch.nan_to_num(lp.abs(), posinf=0.0))
+    same(got.entropy, h, 4 * (rel + 8 * EPS) * (1 + torch.nan_to_num(h)))
+    if top:
+        assert torch.equal(got.top_ids.cpu().long(), tid)
+        same(got.top_logprobs, tlp, rel + 4 * EPS * torch.nan_to_num(tlp.abs(), posinf=0.0))
+    else:
+        assert got.top_ids is None and got.top_logprobs is None
+
+
+def rows(r, v, dtype, seed, gap=0, shift=0, std=2.5, device="cpu"):
+    g = torch.Generator().manual_seed(seed)
+    store = torch.randn(shift + r * (v + gap), generator=g).mul_(std).to(dtype).to(device)
+    return store[shift:].view(r, v + gap)[:, :v], torch.randint(0, v, (r,), generator=g).to(device)
+
+
+def special(v, dtype):
+    """Rows at the edges: shut out in part, but for one token, as a whole, at the type's ends, all equal, infinities, NaN, zeros of both
+    signs."""
+    lowest, highest = torch.finfo(dtype).min, torch.finfo(dtype).max
+    z = torch.randn(13, v, generator=torch.Generator().manual_seed(3)) * 3
+    z[0, ::2] = -INF
+    z[1] = -INF
+    z[1, v // 2] = 1.5
+    z[2] = -INF
+    z[3] = lowest
+    z[4] = lowest
+    z[4, v - 1] = 0.25
+    z[5] = 2.0
+    z[6, v // 3] = INF
+    z[7] = INF
+    z[8, v // 2] = NAN
+    z[9] = torch.where(torch.arange(v) % 3 == 0, -0.0, 0.0)
+    z[10] = lowest
+    z[10, 0] = highest
+    z[11, v - 1] = INF
+    z[11, 0] = -INF
+    z[12] = torch.arange(v) / 64.0
+    return z.to(dtype)
+
+
+@pytest.mark.parametrize("v", [1, 2, 7, 300])
+@pytest.mark.parametrize("top", [0, 1, 5, 32])
+def test_cpu_matches_the_definition(v, top):
+    z, ids = rows(4, v, torch.float32, v)
+    check(z, ids, top, ops.token_logprobs(z, ids, top))
+    z = special(v, torch.float32)
+    ids = torch.randint(-1, v + 1, (13, 3), generator=torch.Generator().manual_seed(1))
+    check(z, ids, top, ops.token_logprobs(z, ids, top))
+
+
+def test_linear_on_cpu_is_the_product_and_its_logprobs():
+    g = torch.Generator().manual_seed(0)
+    x, w = torch.randn(9, 24, generator=g), torch.randn(70, 24, generator=g)
+    ids = torch.randint(0, 70, (9,), generator=g)
+    for cap in (0.0, 2.0):
+        z = x.double() @ w.double().t()
+        z = cap * torch.tanh(z / cap) if cap else z
+        got = ops.linear_logprobs(x, ops.LinearWeight("dense", w), ids, softcap=cap, top=3)
+        lp, h, tid, _ = oracle(z, ids, 3)
+        same(got.logprob, lp, 1e-5)       # 24 products of about 1, rounded to 2^-24 each, in both the row's token and its sum
+        same(got.entropy, h, 1e-4)
+        assert torch.equal(got.top_ids.long(), tid)
+
+
+def test_linear_in_chunks_gives_the_same(monkeypatch):
+    g = torch.Generator().manual_seed(0)
+    x, w = torch.randn(11, 16, generator=g), ops.LinearWeight("dense", torch.randn(40, 16, generator=g))
+    ids = torch.randint(0, 40, (11,), generator=g)
+    whole = ops.linear_logprobs(x, w, ids, top=2)
+    monkeypatch.setattr(LP, "CHUNK_LOGITS", 160)
+    parts = ops.linear_logprobs(x, w, ids, top=2)
+    assert all(torch.allclose(a, b, atol=1e-6) for a, b in zip(whole, parts))
+    none = ops.linear_logprobs(x[:0], w, ids[:0], top=2)
+    assert none.logprob.shape == (0,) and none.top_ids.shape == (0, 2)
+
+
+def test_refusals():
+    z, ids = torch.zeros(3, 8), torch.zeros(3, dtype=torch.int64)
+    w = ops.LinearWeight("dense", torch.zeros(8, 4))
+    for bad in (lambda: ops.token_logprobs(z[0], ids), lambda: ops.token_logprobs(z.double(), ids), lambda: ops.token_logprobs(z.t(), ids),
+                lambda: ops.token_logprobs(z[:, :0], ids), lambda: ops.token_logprobs(z, ids[:2]), lambda: ops.token_logprobs(z, ids.float()),
+                lambda: ops.token_logprobs(z, ids, -1), lambda: ops.token_logprobs(z, ids, 33),
+                lambda: ops.token_logprobs(z, ids.view(3, 1, 1)), lambda: ops.linear_logprobs(torch.zeros(3, 5), w, ids),
+                lambda: ops.linear_logprobs(torch.zeros(3, 4), w, ids.view(3, 1)), lambda: ops.linear_logprobs(torch.zeros(3, 4), w, ids, softcap=-1.0),
+                lambda: ops.linear_logprobs(torch.zeros(3, 4), w, ids, softcap=NAN), lambda: ops.linear_logprobs(torch.zeros(3, 4), w, ids, top=40)):
+        with pytest.raises(ValueError):
+            bad()
+
+
+def test_the_launcher_refuses():
+    """Arguments that the C entry turns into errors before anything is launched."""
+    if not _lib.kernels_available():
+        pytest.skip("the kernel library is not built")
+    f = LP._k().sllm_token_logprobs
+    ok = [256, 8, 3, 8, 0, 256, 1, 1, 4, 256, 256, 256, 256, None]
+    for at, value, code in ((0, None, 1), (1, -1, 1), (2, 0, 1), (3, 0, 1), (4, 3, 1), (5, None, 1), (7, -1, 1), (8, 33, 7), (9, None, 1),
+                            (10, None, 1), (11, None, 1), (12, None, 1), (0, 257, 3)):
+        a = list(ok)
+        a[at] = value
+        assert f(*a) == code, (at, value)
+
+
+# ------------------------------------------------------------------------------------------ kernels
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("r,v,gap,shift,top", [(1, 1, 0, 0, 3), (2, 5, 3, 1, 2), (3, 31, 0, 0, 32), (5, 257, 1, 1, 1), (4, 2048, 0, 0, 5),
+                                               (7, 4099, 5, 3, 20), (1, 32000, 0, 0, 32), (300, 1000, 24, 8, 4), (700, 515, 0, 1, 0), (2, 131077, 11, 7, 20),
+                                               (160, 9001, 0, 0, 7)])
+def test_kernel_matches_the_definition(dtype, r, v, gap, shift, top):
+    z, ids = rows(r, v, dtype, r * v, gap, shift, device=DEV)
+    check(z, ids, top, ops.token_logprobs(z, ids.int() if r % 2 else ids, top))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("v", [1, 2, 33, 1000, 20011])
+@pytest.mark.parametrize("top", [0, 6, 32])
+def test_kernel_at_the_edges(dtype, v, top):
+    z = special(v, dtype).to(DEV)
+    ids = torch.randint(-1, v + 1, (13, 3), generator=torch.Generator().manual_seed(1)).to(DEV)
+    check(z, ids, top, ops.token_logprobs(z, ids, top))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("order", ["rising", "falling", "equal", "runs", "few"])
+@pytest.mark.parametrize("v", [700, 40000])
+def test_alternatives_of_ordered_rows(order, v):
+    """Rows in which many tokens pass for candidates: sorted ones, ties of all or most of the row, fewer tokens than alternatives."""
+    i = torch.arange(v)
+    z = {"rising": i * 0.5, "falling": -i * 0.5, "equal": i * 0.0, "runs": (i // 97 % 5) * 1.0,
+         "few": torch.where(i % (v // 3) == 1, i * 1.0, torch.tensor(-INF))}[order]
+    z = torch.stack([z, z.flip(0)]).to(DEV)
+    ids = torch.tensor([0, v - 1], device=DEV)
+    for x in (z, z.bfloat16()):
+        got = ops.token_logprobs(x, ids, 32)
+        _, _, tid, _ = oracle(x, ids, 32)
+        assert torch.equal(got.top_ids.cpu().long(), tid)
+
+
+@pytest.mark.gpu
+def test_rows_whose_offsets_pass_32_bits():
+    store = torch.empty((1 << 31) + 5000, dtype=torch.bfloat16, device=DEV)
+    z = store.as_strided((2, 4100), (1 << 31, 1), 3)
+    z.copy_(torch.randn(2, 4100, generator=torch.Generator().manual_seed(0)))
+    ids = torch.tensor([[0, 4099], [17, 4098]], device=DEV)
+    check(z, ids, 5, ops.token_logprobs(z, ids, 5))
+
+
+@pytest.mark.gpu
+def test_broadcast_rows_streams_and_graphs():
+    z, ids = rows(6, 5003, torch.bfloat16, 0, device=DEV)
+    one = z[:1].expand(6, -1)
+    check(one, ids, 3, ops.token_logprobs(one, ids, 3))
+    want = ops.token_logprobs(z, ids, 3)
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        a = ops.token_logprobs(z, ids, 3)
+    b = ops.token_logprobs(z, ids, 3)                       # two calls at once
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, w) and torch.equal(q, w) for p, q, w in zip(a, b, want))
+    static, g = z.clone(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = ops.token_logprobs(static, ids, 3)
+    static.copy_(z.flip(0))
+    g.replay()
+    want = ops.token_logprobs(z.flip(0), ids, 3)
+    assert all(torch.equal(p, w) for p, w in zip(got, want))
+
+
+@pytest.mark.gpu
+def test_no_rows():
+    got = ops.token_logprobs(torch.empty((0, 9), device=DEV), torch.empty(0, dtype=torch.int32, device=DEV), 2)
+    assert got.logprob.shape == (0,) and got.top_ids.shape == (0, 2)
+    got = ops.token_logprobs(torch.zeros((2, 9), device=DEV), torch.empty((2, 0), dtype=torch.int32, device=DEV))
+    assert got.logprob.shape == (2, 0) and torch.allclose(got.entropy.cpu(), torch.tensor(math.log(9.0)))
+
+
+def head_case(r, d, v, seed, std=2.5):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn((r, d), generator=g).bfloat16()
+    w = (torch.randn((v, d), generator=g) * std / math.sqrt(d)).bfloat16()
+    return x.to(DEV), w.to(DEV), torch.randint(0, v, (r,), generator=g, dtype=torch.int32).to(DEV)
+
+
+def head_check(x, w, ids, cap, got, extra=0):
+    """A logit is a sum of d exact products: every 16 of them are added with one rounding towards zero (2^-23 of a partial sum, which
+    is at most the sum of magnitudes), so it is off by d / 16 + 8 such roundings; log p moves by the errors of the token's logit and of
+    the weighted logits, H by the logits' errors times 2 (1 + spread of the logits)."""
+    z = x.double() @ w.double().t()
+    mag = (x.double().abs() @ w.double().abs().t()).max()
+    dz = float(mag) * (x.shape[1] / 16 + 8) * 2 ** -23
+    if cap:
+        z = cap * torch.tanh(z / cap)
+    lp, h, _, _ = oracle(z, ids, 0)
+    spread = float(z.max() - z.min())
+    rel = (w.shape[0] / 256 + 64) * EPS
+    same(got.logprob, lp, 2 * dz + rel + 8 * EPS * (lp.abs() + cap))
+    same(got.entropy, h, 2 * (dz + 8 * EPS * cap) * (1 + spread) + 4 * rel * (1 + h))
+
+
+HEADS = [(1, 8, 1), (1, 64, 300), (3, 72, 1000), (16, 512, 2048), (17, 128, 777), (128, 64, 257), (129, 200, 1025), (300, 1024, 5000), (513, 8, 40),
+         (40, 4096, 3001)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cap", [0.0, 5.0])
+@pytest.mark.parametrize("r,d,v", HEADS)
+def test_head_matches_the_definition(r, d, v, cap):
+    x, w, ids = head_case(r, d, v, r + d + v)
+    head_check(x, w, ids, cap, ops.linear_logprobs(x, ops.LinearWeight("dense", w), ids, softcap=cap))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,v", [(12, 50), (33, 300)])
+def test_head_of_odd_widths_and_fp32(d, v):
+    x, w, ids = head_case(5, d, v, 1)
+    head_check(x, w, ids, 0.0, ops.linear_logprobs(x, ops.LinearWeight("dense", w), ids))
+    head_check(x, w, ids, 0.0, ops.linear_logprobs(x.float(), ops.LinearWeight("dense", w.float()), ids))
+
+
+@pytest.mark.gpu
+def test_head_with_alternatives_and_quantised_weights():
+    x, w, ids = head_case(40, 256, 3000, 2)
+    got = ops.linear_logprobs(x, ops.LinearWeight("dense", w), ids, top=4)
+    z = ops.linear(x, ops.LinearWeight("dense", w), out_fp32=True)
+    want = ops.token_logprobs(z, ids, 4)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    fp8 = ops.LinearWeight.from_dense(w.cpu().float(), "fp8").to(DEV)
+    for rows_ in (x, ops.quant_fp8(x)):
+        got = ops.linear_logprobs(rows_, fp8, ids, top=4)
+        want = ops.token_logprobs(ops.linear(rows_, fp8), ids, 4)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
