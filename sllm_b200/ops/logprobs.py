@@ -15,6 +15,7 @@ _SIGS = {
 }
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 MAX_TOP = 32
+MAX_VOCAB = 1 << 30
 CHUNK_LOGITS = 1 << 26         # logits that `linear_logprobs` holds at a time where it writes them
 
 
@@ -74,8 +75,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     any stride), the rows' entropies and their ``top`` (0 to 32) likeliest tokens.  -inf logits are shut out: a row of nothing else has
     log-probabilities of -inf, entropy 0 and no alternatives.  A row with +inf is uniform over those; one with NaN gives NaN and no
     alternatives.  A token below 0 stands for none (0, so that padded places drop out of sums), one from V on gives NaN."""
-    if logits.dim() != 2 or logits.dtype not in _DTYPES or logits.shape[1] < 1 or (logits.shape[1] > 1 and logits.stride(1) != 1):
-        raise ValueError("logits are bf16, fp16 or fp32 [rows, vocabulary] with contiguous rows")
+    if (logits.dim() != 2 or logits.dtype not in _DTYPES or not 1 <= logits.shape[1] <= MAX_VOCAB
+            or (logits.shape[1] > 1 and logits.stride(1) != 1)):
+        raise ValueError(f"logits are bf16, fp16 or fp32 [rows, vocabulary] with contiguous rows of at most {MAX_VOCAB}")
     if not 0 <= top <= MAX_TOP:
         raise ValueError(f"top lies between 0 and {MAX_TOP}")
     _check_tokens(tokens, logits.shape[0], logits.device)

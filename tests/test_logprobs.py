@@ -150,7 +150,7 @@ def test_the_launcher_refuses():
         pytest.skip("the kernel library is not built")
     f = LP._k().sllm_token_logprobs
     ok = [256, 8, 3, 8, 0, 256, 1, 1, 4, 256, 256, 256, 256, None]
-    for at, value, code in ((0, None, 1), (1, -1, 1), (2, 0, 1), (3, 0, 1), (4, 3, 1), (5, None, 1), (7, -1, 1), (8, 33, 7), (9, None, 1),
+    for at, value, code in ((0, None, 1), (1, -1, 1), (2, 0, 1), (3, 0, 1), (3, (1 << 30) + 1, 7), (4, 3, 1), (5, None, 1), (7, -1, 1), (8, 33, 7), (9, None, 1),
                             (10, None, 1), (11, None, 1), (12, None, 1), (0, 257, 3)):
         a = list(ok)
         a[at] = value
