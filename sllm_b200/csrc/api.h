@@ -96,6 +96,12 @@ int sllm_token_logprobs(const void* logits, long long ld, int rows, int vocab, i
                         int tokens64, int given, int top, float* logprob, float* entropy, int* top_ids,
                         float* top_logprobs, void* stream);
 
+/* head_logprobs.cu */
+long long sllm_head_logprobs_floats(int m, int n, int bn);
+int sllm_head_logprobs(const void* x, const void* w, const int* tokens, int m, int n, int k, long long ldx, float cap,
+                       int bn, float* ws, long long ws_floats, float* logprob, float* entropy, int* status,
+                       void* stream);
+
 /* batch_plan.cu */
 int sllm_batch_plan(const int* new_lens, const int* starts, const int* pages, long long page_count, int requests,
                     int rows, int max_blocks, long long ld_table, int page, int* row_off, int* positions,

@@ -54,14 +54,46 @@ __device__ __forceinline__ float lp_max(const LpVec<T>& v) {   // of what is no 
     return fmaxf(m.x, m.y);
   }
 }
+__device__ __forceinline__ uint32_t lp_word(const uint4& r, int i) { return i == 0 ? r.x : i == 1 ? r.y : i == 2 ? r.z : r.w; }
+template <typename T>
+__device__ __forceinline__ float2 lp_split(uint32_t w) {       // of 16-bit types
+  if constexpr (std::is_same_v<T, __half>) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
 template <typename T>
 __device__ __forceinline__ float2 lp_pair(const LpVec<T>& v, int i) {
+  if constexpr (sizeof(T) == 4) return make_float2(__uint_as_float(lp_word(v.raw, 2 * i)), __uint_as_float(lp_word(v.raw, 2 * i + 1)));
+  else return lp_split<T>(lp_word(v.raw, i));
+}
+
+// Sums are taken in powers of two, t = z log2(e) - m2 with m2 the rounded product of the reference: S = sum 2^t and W = sum 2^t t.
+// Logits below kLow (-inf and masks of the type's lowest value) count as it, so that 2^t t is 0 and no NaN; where a row's largest
+// logit is not well above it, or beyond kHigh, the sums are taken anew from exact differences (`lp_wide`).
+template <typename T>
+struct LpRange {
+  static constexpr bool kHalf = std::is_same_v<T, __half>;
+  static constexpr float kLow = kHalf ? -60000.f : -7.9228163e28f;      // (-2^96)
+  static constexpr float kWide = kHalf ? -59000.f : -3.9614081e28f;     // (-2^95)
+  static constexpr float kHigh = 3.9614081e28f;
+  static constexpr uint32_t kLowPair = kHalf ? 0xfb53fb53u : 0xef80ef80u;
+};
+template <typename T>
+__device__ __forceinline__ bool lp_wide(float m) { return !(m > LpRange<T>::kWide && m < LpRange<T>::kHigh); }
+__device__ __forceinline__ float lp_max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ float2 lp_pair_from_low(const LpVec<T>& v, int i) {      // lp_pair, nothing below kLow
   if constexpr (sizeof(T) == 4) {
-    return i == 0 ? make_float2(__uint_as_float(v.raw.x), __uint_as_float(v.raw.y)) : make_float2(__uint_as_float(v.raw.z), __uint_as_float(v.raw.w));
+    const float2 x = lp_pair(v, i);
+    return make_float2(lp_max_nan(x.x, LpRange<T>::kLow), lp_max_nan(x.y, LpRange<T>::kLow));
   } else {
-    const uint32_t w = i == 0 ? v.raw.x : i == 1 ? v.raw.y : i == 2 ? v.raw.z : v.raw.w;
-    if constexpr (std::is_same_v<T, __half>) return __half22float2(*reinterpret_cast<const __half2*>(&w));
-    else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    uint32_t w;
+    if constexpr (LpRange<T>::kHalf) asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(w) : "r"(lp_word(v.raw, i)), "r"(LpRange<T>::kLowPair));
+    else asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(w) : "r"(lp_word(v.raw, i)), "r"(LpRange<T>::kLowPair));
+    return lp_split<T>(w);
   }
 }
 
@@ -78,11 +110,17 @@ __device__ __forceinline__ float lp_key_value(LpKey k) {
   return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
 }
 // A warp's 32 keys, lane 0 the largest: one exchange of a bitonic network, the whole sort, and the 32 largest of two sorted lists.
+// (Floats hold no NaN.)
 __device__ __forceinline__ LpKey lp_exchange(LpKey k, int dist, bool keep_max) {
   const LpKey o = __shfl_xor_sync(0xffffffffu, k, dist);
   return (k > o) == keep_max ? k : o;
 }
-__device__ __forceinline__ LpKey lp_sort(LpKey k) {
+__device__ __forceinline__ float lp_exchange(float k, int dist, bool keep_max) {
+  const float o = __shfl_xor_sync(0xffffffffu, k, dist);
+  return keep_max ? fmaxf(k, o) : fminf(k, o);
+}
+template <typename K>
+__device__ __forceinline__ K lp_sort(K k) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int size = 2; size <= 32; size *= 2)
@@ -104,58 +142,76 @@ __device__ __forceinline__ float lp_exp2(float x) {            // 0 below the sm
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-__device__ __forceinline__ float lp_max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
 __device__ __forceinline__ uint64_t lp_add2(uint64_t a, uint64_t b) {
   uint64_t d;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
 
-constexpr float kLpLog2e = 1.4426950408889634f;
-constexpr float kLpFloor = -200.f;         // differences below it count as it: e^-200 is 0 in fp32, and 0 times it is no NaN
+// A load that stays where it is written, so that several are under way at a time; the row passes L1 by.
+__device__ __forceinline__ uint4 lp_stream(const uint4* p) {
+  uint4 r;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+  return r;
+}
+
+constexpr float kLpLog2e = 1.4426950408889634f, kLpLn2 = 0.6931471805599453f;
 constexpr float kLpSlack = 4.f;            // a thread's sums are taken anew when a logit passes their reference by more
+
 constexpr int kLpMaxCluster = 8;
 constexpr int kLpSmallUnits = 1024;
-constexpr int kLpFill = 592;
+constexpr int kLpFill = 1184;
 constexpr int kLpMaxVocab = 1 << 30;       // ids and units stay below 2^31
 
-// Sums of one part of a row: reference m, S and W as above with respect to it.
+// Sums of one part of a row with respect to m.
 struct LpStats {
   float m, s, w;
-  __device__ __forceinline__ void rebase(float to) {           // to >= m
-    const float d = fmaxf(m - to, kLpFloor), e = lp_exp2(d * kLpLog2e);
-    w = e * (w + d * s);
+  __device__ __forceinline__ void shift(float t) {             // by 2^t, t <= 0 and finite
+    const float e = lp_exp2(t);
+    w = e * fmaf(t, s, w);
     s *= e;
-    m = to;
+  }
+  __device__ __forceinline__ void add(const LpStats& o) {      // (of the same m; NaN passes through)
+    s += o.s;
+    w += o.w;
+  }
+  // the same with respect to another part's maximum
+  template <typename T>
+  __device__ __forceinline__ LpStats to(float max) const {
+    LpStats r = *this;
+    if (m == max) return r;
+    const float t = lp_wide<T>(m) || lp_wide<T>(max) ? (m - max) * kLpLog2e : __fmul_rn(m, kLpLog2e) - __fmul_rn(max, kLpLog2e);
+    r.m = max;
+    r.shift(fmaxf(t, -1000.f));
+    return r;
   }
 };
+
+constexpr int kLpPool = 256;               // candidates that are ranked against one another
 
 template <int kThreads>
 struct __align__(16) LpShared {
   static constexpr int kWarps = kThreads / 32;
   LpStats stat[kWarps];
-  float best[kWarps];
-  LpKey list[kWarps][32];
-  LpKey found[32];
-  int count;
+  float high[32];                          // the largest of the threads' maxima of each warp
+  int wins, count;
+  unsigned char win[kThreads];             // threads with logits at or above the bound
+  LpKey pool[kLpPool];
+  LpKey merged[kWarps][32];
+  LpKey list[32];                          // the CTA's alternatives
   LpStats part[kLpMaxCluster];             // of the first CTA: what the CTAs of a row found
-  float part_best[kLpMaxCluster];
   LpKey part_list[kLpMaxCluster][32];
-  int bad[2];
+  int inf, nan;
 };
 
 // A cluster of CTAs per row (one where there are many rows), each with a range of the row's 16-byte units; unit v of a range goes to
 // thread v mod kThreads.  One pass takes S and W per thread with respect to a reference that follows the maximum loosely, so that the
 // usual unit has no branch, and the thread's largest logit.
-// Alternatives: the top-th largest of the threads' maxima bounds the wanted ones from below, and only as many threads have
-// logits above it as there are alternatives; those threads' units are read again (out of L2) and what passes the bound is sorted by one warp.
-// Where more than 32 pass it (runs of equal or ordered logits), sorted lists are merged 32 at a time instead.
+// Alternatives: the top-th largest of the threads' maxima bounds the wanted ones from below, and hardly more threads have logits at or
+// above it than there are alternatives; those threads' units are read again (out of L2) and what passes the bound is ranked by
+// counting.  Where more than kLpPool logits pass it (runs of equal or ordered ones), sorted lists are merged 32 at a time instead.
 template <typename T, int kThreads, bool kTop>
-__global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobParams p, int cluster) {
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(const LogprobParams p, int cluster) {
   constexpr int kN = LpVec<T>::kN, kWarps = kThreads / 32, kAhead = 4;
   __shared__ LpShared<kThreads> sh;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
@@ -189,46 +245,44 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobParams 
     }
     return u;
   };
-  // the given tokens' logits, ahead of the pass
+  // the given tokens: ids ahead of the pass, their logits behind it
   const float nan = __int_as_float(0x7fffffff);
-  auto given = [&](int j, long long& id) {
+  auto token = [&](int j) {
     const long long at = row * p.given + j;
-    id = p.tokens64 ? static_cast<const long long*>(p.tokens)[at] : static_cast<const int*>(p.tokens)[at];
-    return id >= 0 && id < p.vocab ? lp_load(z + id) : 0.f;
+    return p.tokens64 ? static_cast<const long long*>(p.tokens)[at] : static_cast<long long>(static_cast<const int*>(p.tokens)[at]);
   };
+  auto logit = [&](long long id) { return id >= 0 && id < p.vocab ? lp_load(z + id) : 0.f; };
   long long tok = -1;
-  float tok_x = 0.f;
-  if (rank == 0 && tid < p.given) tok_x = given(tid, tok);
+  if (rank == 0 && tid < p.given) tok = token(tid);
 
-  LpStats st = {-FLT_MAX, 0.f, 0.f};
-  float best = kNone;
-  int best_at = 0;
+  float best = kNone;                                          // the thread's largest logit
+  float limit = LpRange<T>::kLow, m2 = LpRange<T>::kLow * kLpLog2e;      // reference of its sums, as the logit that asks for another one and as m2
   uint64_t s2 = 0ull, w2 = 0ull;
-  auto add = [&](const LpVec<T>& u, int v) {
+  auto add = [&](const LpVec<T>& u) {
     const float top = lp_max(u);
-    if constexpr (kTop) best_at = top > best ? v : best_at;
     best = fmaxf(best, top);
-    if (top > st.m + kLpSlack) {
+    if (top > limit) {
       const float2 s = unpack_f32x2(s2), w = unpack_f32x2(w2);
-      st.s = s.x + s.y;
-      st.w = w.x + w.y;
-      st.rebase(top);
+      const float next = top * kLpLog2e;
+      LpStats st = {0.f, s.x + s.y, w.x + w.y};
+      st.shift(m2 - next);
       s2 = pack_f32x2(st.s, 0.f);
       w2 = pack_f32x2(st.w, 0.f);
+      m2 = next;
+      limit = top + kLpSlack;
     }
-    const uint64_t ref = pack_f32x2(-st.m, -st.m), scale = pack_f32x2(kLpLog2e, kLpLog2e);
+    const uint64_t ref = pack_f32x2(-m2, -m2), scale = pack_f32x2(kLpLog2e, kLpLog2e);
 #pragma unroll
     for (int i = 0; i < kN / 2; ++i) {
-      const float2 x = lp_pair(u, i);
-      float2 d = unpack_f32x2(lp_add2(pack_f32x2(x.x, x.y), ref));
-      const uint64_t d2 = pack_f32x2(lp_max_nan(d.x, kLpFloor), lp_max_nan(d.y, kLpFloor));
-      const float2 t = unpack_f32x2(mul_f32x2(d2, scale));
+      const float2 x = lp_pair_from_low(u, i);
+      const uint64_t t2 = fma_f32x2(pack_f32x2(x.x, x.y), scale, ref);
+      const float2 t = unpack_f32x2(t2);
       const uint64_t e2 = pack_f32x2(lp_exp2(t.x), lp_exp2(t.y));
       s2 = lp_add2(s2, e2);
-      w2 = fma_f32x2(e2, d2, w2);
+      w2 = fma_f32x2(e2, t2, w2);
     }
   };
-  if (lo + tid < min(hi, whole_lo)) add(load_unit(lo + tid), lo + tid);
+  if (lo + tid < min(hi, whole_lo)) add(load_unit(lo + tid));
   // (whole_lo is at most 1: only thread 0 of the first range has such a unit, and goes on behind it)
   const int end = min(hi, whole_hi);
   for (int v = lo + tid + (lo + tid < whole_lo ? kThreads : 0); v < end; v += kAhead * kThreads) {
@@ -236,120 +290,155 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobParams 
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       u[i].raw = make_uint4(lp_shut<T>(), lp_shut<T>(), lp_shut<T>(), lp_shut<T>());
-      if (v + i * kThreads < end) u[i].raw = units[v + i * kThreads];
+      if (v + i * kThreads < end) u[i].raw = lp_stream(units + v + i * kThreads);
     }
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) add(u[i], v + i * kThreads);
+    for (int i = 0; i < kAhead; ++i) add(u[i]);
   }
   {
     const int v = n_units - 1;                                 // the last unit, where it is not whole and was not the first as well
-    if (v >= whole_hi && v >= whole_lo && v >= lo && v < hi && (v - lo) % kThreads == tid) add(load_unit(v), v);
+    if (v >= whole_hi && v >= whole_lo && v >= lo && v < hi && (v - lo) % kThreads == tid) add(load_unit(v));
   }
 
-  // the CTA's sums
+  float tok_x = logit(tok);
+
+  // the CTA's sums: the threads' of each warp with respect to the warp's maximum, then the warps'
+  auto join = [&](const LpStats* part, int parts) {
+    float m = part[0].m;
+    for (int i = 1; i < parts; ++i) m = fmaxf(m, part[i].m);
+    LpStats all = {m, 0.f, 0.f};
+    for (int i = 0; i < parts; ++i) all.add(part[i].to<T>(m));
+    return all;
+  };
   {
     const float2 s = unpack_f32x2(s2), w = unpack_f32x2(w2);
-    st.s = s.x + s.y;
-    st.w = w.x + w.y;
+    LpStats st = {warp_max(best), s.x + s.y, w.x + w.y};
+    // (a warp without logits above kLow leaves a sum that `to` takes away; t is not finite only where the row is taken anew)
+    st.shift(m2 - __fmul_rn(fmaxf(st.m, LpRange<T>::kLow), kLpLog2e));
+    st.s = warp_sum(st.s);
+    st.w = warp_sum(st.w);
+    if (lane == 0) sh.stat[warp] = st;
+    if (tid == 0) sh.inf = sh.nan = sh.count = sh.wins = 0;
   }
-  const float warp_best = warp_max(best);
-  if (lane == 0) sh.best[warp] = warp_best;
-  if (tid == 0) sh.bad[0] = sh.bad[1] = sh.count = 0;
   __syncthreads();
-  float all_best = sh.best[0];
+  bool again = false;
+  {
+    float m = kNone;
 #pragma unroll
-  for (int w = 1; w < kWarps; ++w) all_best = fmaxf(all_best, sh.best[w]);
-  const bool odd = !(all_best < INFINITY) || st.s != st.s;     // +inf or NaN among the logits
-  if (__syncthreads_or(odd)) {
+    for (int w = 0; w < kWarps; ++w) {
+      m = fmaxf(m, sh.stat[w].m);
+      again |= !(sh.stat[w].s < INFINITY);
+    }
+    if (lp_wide<T>(m)) again = true;
+  }
+  LpStats mine;
+  if (!again) {
+    mine = join(sh.stat, kWarps);
+  } else {
+    float m = sh.stat[0].m;
+    for (int w = 1; w < kWarps; ++w) m = fmaxf(m, sh.stat[w].m);
+    LpStats st = {m, 0.f, 0.f};
     int inf = 0, bad = 0;
     for (int v = lo + tid; v < hi; v += kThreads) {
       const LpVec<T> u = load_unit(v);
 #pragma unroll
-      for (int i = 0; i < kN / 2; ++i) {
-        const float2 x = lp_pair(u, i);
-        inf += (x.x == INFINITY) + (x.y == INFINITY);
-        bad += (x.x != x.x) + (x.y != x.y);
+      for (int i = 0; i < kN; ++i) {
+        const float2 x = lp_pair(u, i / 2);
+        const float y = i & 1 ? x.y : x.x;
+        inf += y == INFINITY;
+        bad += y != y;
+        if (y > -INFINITY && m < INFINITY) {
+          const float t = fmaxf((y == m ? 0.f : y - m) * kLpLog2e, -1000.f), e = lp_exp2(t);
+          st.s += e;
+          st.w += e * t;
+        }
       }
     }
-    if (inf) atomicAdd(&sh.bad[0], inf);
-    if (bad) atomicAdd(&sh.bad[1], bad);
+    st.s = warp_sum(st.s);
+    st.w = warp_sum(st.w);
+    inf = __reduce_add_sync(0xffffffffu, inf);
+    bad = __reduce_add_sync(0xffffffffu, bad);
     __syncthreads();
-    // uniform over +inf: every one counts 1, with no difference to the maximum
-    st.m = all_best;
-    st.s = tid == 0 ? (sh.bad[1] ? nan : static_cast<float>(sh.bad[0])) : 0.f;
-    st.w = 0.f;
-  } else {
-    st.rebase(fmaxf(all_best, -FLT_MAX));
-  }
-  st.s = warp_sum(st.s);
-  st.w = warp_sum(st.w);
-  if (lane == 0) sh.stat[warp] = st;
-  __syncthreads();
-  LpStats mine = sh.stat[0];
-#pragma unroll
-  for (int w = 1; w < kWarps; ++w) {
-    mine.s += sh.stat[w].s;
-    mine.w += sh.stat[w].w;
+    if (lane == 0) {
+      sh.stat[warp] = st;
+      atomicAdd(&sh.inf, inf);
+      atomicAdd(&sh.nan, bad);
+    }
+    __syncthreads();
+    mine = {m, 0.f, 0.f};
+    for (int w = 0; w < kWarps; ++w) mine.add(sh.stat[w]);
+    if (sh.inf) mine = {m, static_cast<float>(sh.inf), 0.f};   // uniform over +inf
+    if (sh.nan) mine.s = nan;
   }
 
-  LpKey key = 0;                                               // lane i of warp 0: the CTA's i-th alternative
   if constexpr (kTop) {
-    // the thread's maximum stands for the last place of its unit, which orders it rightly against other units
-    key = lp_sort(lp_key(best, best_at * kN + kN - 1 - shift));
-#pragma unroll
-    for (int half = kWarps / 2; half > 0; half /= 2) {
-      if (warp >= half && warp < 2 * half) sh.list[warp][lane] = key;
-      __syncthreads();
-      if (warp < half) key = lp_merge(key, sh.list[warp + half][lane]);
-    }
-    if (warp == 0) sh.found[lane] = lane < p.top ? key : 0;
+    // the bound: top-th largest among the first 32 / kWarps maxima of each warp, which leaves hardly more than the wanted ones above it
+    constexpr int kHigh = 32 / kWarps;
+    const float v = lp_sort(best);
+    if (lane < kHigh) sh.high[warp * kHigh + lane] = v;
     __syncthreads();
-    const LpKey bound = sh.found[p.top - 1];                   // 0: every token counts
-    LpKey mine_k = 0;
-    // what passes the bound among a winner's units, one place of the units at a time
-    auto scan = [&](auto&& take) {
-      for (int j = warp; j < p.top; j += kWarps) {
-        const LpKey win = sh.found[j];
-        if (!win) break;
-        const int owner = ((lp_key_id(win) - (kN - 1) + shift) / kN - lo) % kThreads;
-        for (int v0 = lo + owner; v0 < hi; v0 += 32 * kThreads) {
-          const int v = v0 + lane * kThreads;
-          LpVec<T> u;
-          u.raw = make_uint4(lp_shut<T>(), lp_shut<T>(), lp_shut<T>(), lp_shut<T>());
-          if (v < hi) u = load_unit(v);
+    const float bound = __shfl_sync(0xffffffffu, lp_sort(sh.high[lane]), p.top - 1);      // -inf: every token counts
+    if (best >= bound && best > -INFINITY) sh.win[atomicAdd(&sh.wins, 1)] = static_cast<unsigned char>(tid);
+    __syncthreads();
+    // the winners' units, dealt out over all threads
+    const int each = (hi - lo + kThreads - 1) / kThreads, todo = sh.wins * each;
+    auto unit_of = [&](int i) { return i < todo ? lo + sh.win[i / each] + i % each * kThreads : hi; };      // hi: none
+    for (int i0 = tid; i0 < todo; i0 += kAhead * kThreads) {
+      LpVec<T> u[kAhead];
+      int at[kAhead];
 #pragma unroll
-          for (int i = 0; i < kN; ++i) {
-            const float2 x = lp_pair(u, i / 2);
-            const LpKey k = lp_key(i & 1 ? x.y : x.x, v * kN + i - shift);
-            take(k >= bound ? k : 0);
+      for (int i = 0; i < kAhead; ++i) {
+        at[i] = unit_of(i0 + i * kThreads);
+        u[i].raw = make_uint4(lp_shut<T>(), lp_shut<T>(), lp_shut<T>(), lp_shut<T>());
+        if (at[i] < hi) u[i] = load_unit(at[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        if (!(lp_max(u[i]) >= bound)) continue;
+#pragma unroll
+        for (int e = 0; e < kN; ++e) {
+          const float2 x = lp_pair(u[i], e / 2);
+          const float y = e & 1 ? x.y : x.x;
+          if (y >= bound && y > -INFINITY) {
+            const int n = atomicAdd(&sh.count, 1);
+            if (n < kLpPool) sh.pool[n] = lp_key(y, at[i] * kN + e - shift);
           }
         }
       }
-    };
-    LpKey* pool = &sh.list[0][0];                              // 32 keys at least
-    scan([&](LpKey k) {
-      if (k) {
-        const int at = atomicAdd(&sh.count, 1);
-        if (at < 32) pool[at] = k;
-      }
-    });
+    }
+    if (tid < 32) sh.list[tid] = 0;
     __syncthreads();
-    if (sh.count <= 32) {
-      if (warp == 0) key = lp_sort(lane < sh.count ? pool[lane] : 0);
+    const int count = sh.count;
+    if (count <= kLpPool) {
+      for (int i = tid; i < count; i += kThreads) {
+        const LpKey k = sh.pool[i];
+        int place = 0;
+        for (int j = 0; j < count; ++j) place += sh.pool[j] > k;
+        if (place < p.top) sh.list[place] = k;
+      }
     } else {
-      scan([&](LpKey k) {
-        const LpKey least = __shfl_sync(0xffffffffu, mine_k, 31);
-        if (__any_sync(0xffffffffu, k > least)) mine_k = lp_merge(mine_k, lp_sort(k));
-      });
-      __syncthreads();
-      key = mine_k;
+      LpKey best_k = 0;                                        // the warp's 32 largest, lane 0 the first
+      for (int i0 = warp * 32; i0 < todo; i0 += kThreads) {
+        const int at = unit_of(i0 + lane);
+        LpVec<T> u;
+        u.raw = make_uint4(lp_shut<T>(), lp_shut<T>(), lp_shut<T>(), lp_shut<T>());
+        if (at < hi) u = load_unit(at);
+#pragma unroll
+        for (int e = 0; e < kN; ++e) {
+          const float2 x = lp_pair(u, e / 2);
+          const LpKey k = lp_key(e & 1 ? x.y : x.x, at * kN + e - shift), least = __shfl_sync(0xffffffffu, best_k, 31);
+          if (__any_sync(0xffffffffu, k > least)) best_k = lp_merge(best_k, lp_sort(k));
+        }
+      }
 #pragma unroll
       for (int half = kWarps / 2; half > 0; half /= 2) {
-        if (warp >= half && warp < 2 * half) sh.list[warp][lane] = key;
+        if (warp >= half && warp < 2 * half) sh.merged[warp][lane] = best_k;
         __syncthreads();
-        if (warp < half) key = lp_merge(key, sh.list[warp + half][lane]);
+        if (warp < half) best_k = lp_merge(best_k, sh.merged[warp + half][lane]);
       }
+      if (warp == 0) sh.list[lane] = lane < p.top ? best_k : 0;
     }
+    __syncthreads();
   }
 
   if (cluster > 1) {
@@ -358,7 +447,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobParams 
     uint32_t to;
     if (kTop && warp == 0) {
       asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to) : "r"(smem_u32(&sh.part_list[rank][lane])));
-      asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(to), "l"(key) : "memory");
+      asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(to), "l"(sh.list[lane]) : "memory");
     }
     if (tid == 0) {
       asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to) : "r"(smem_u32(&sh.part[rank])));
@@ -369,36 +458,37 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobParams 
     __syncwarp();
     cluster_sync_pair();
     if (rank != 0) return;
-    float m = sh.part[0].m;
-    for (int c = 1; c < cluster; ++c) m = fmaxf(m, sh.part[c].m);
-    mine = {m, 0.f, 0.f};
-    for (int c = 0; c < cluster; ++c) {
-      LpStats q = sh.part[c];
-      if (q.m == m) {                                          // (+inf: the parts without one have nothing to add)
-        mine.s += q.s;
-        mine.w += q.w;
-      } else {
-        q.rebase(m);
-        mine.s += q.s;                                         // a NaN of any part passes through
-        mine.w += q.w;
+    mine = join(sh.part, cluster);
+    if constexpr (kTop) {                                      // the CTAs' lists, two by two
+      for (int gap = 1; gap < cluster; gap *= 2) {
+        const int c = 2 * gap * warp;
+        if (c + gap < cluster) sh.part_list[c][lane] = lp_merge(sh.part_list[c][lane], sh.part_list[c + gap][lane]);
+        __syncthreads();
       }
-    }
-    if (kTop && warp == 0) {
-      key = sh.part_list[0][lane];
-      for (int c = 1; c < cluster; ++c) key = lp_merge(key, sh.part_list[c][lane]);
+      if (tid < 32) sh.list[tid] = sh.part_list[0][tid];
+      __syncthreads();
     }
   }
-  const float ln_s = logf(mine.s);
-  const bool bad = mine.s != mine.s;
-  auto logp = [&](float x) { return bad ? nan : x > -INFINITY ? (x == mine.m ? 0.f : x - mine.m) - ln_s : -INFINITY; };
-  if (tid == 0) p.entropy[row] = bad ? nan : mine.s > 0.f ? ln_s - mine.w / mine.s : 0.f;
+  const float log_s = log2f(mine.s);
+  const bool bad = mine.s != mine.s, wide = lp_wide<T>(mine.m);
+  auto logp = [&](float x) {
+    if (bad) return nan;
+    if (!(x > -INFINITY)) return -INFINITY;
+    if (wide || lp_wide<T>(x)) return (x == mine.m ? 0.f : x - mine.m) - log_s * kLpLn2;
+    return (fmaf(x, kLpLog2e, -__fmul_rn(mine.m, kLpLog2e)) - log_s) * kLpLn2;
+  };
+  if (tid == 0) p.entropy[row] = bad ? nan : mine.s > 0.f ? (log_s - mine.w / mine.s) * kLpLn2 : 0.f;
   for (int j = tid; j < p.given; j += kThreads) {
-    if (j != tid) tok_x = given(j, tok);
+    if (j != tid) {
+      tok = token(j);
+      tok_x = logit(tok);
+    }
     p.logprob[row * p.given + j] = tok < 0 ? 0.f : tok >= p.vocab ? nan : logp(tok_x);
   }
-  if (kTop && warp == 0 && lane < p.top) {
-    p.top_ids[row * p.top + lane] = key && !bad ? lp_key_id(key) : -1;
-    p.top_logprobs[row * p.top + lane] = bad ? nan : key ? logp(lp_key_value(key)) : -INFINITY;
+  if (kTop && tid < p.top) {
+    const LpKey key = bad ? 0 : sh.list[tid];
+    p.top_ids[row * p.top + tid] = key ? lp_key_id(key) : -1;
+    p.top_logprobs[row * p.top + tid] = bad ? nan : key ? logp(lp_key_value(key)) : -INFINITY;
   }
 }
 

@@ -8,21 +8,24 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib
+from .core import _launch
 
 P, I, L = C.c_void_p, C.c_int, C.c_longlong
 _SIGS = {
     "sllm_token_logprobs": (I, [P, L, I, I, I, P, I, I, I, P, P, P, P, P]),
+    "sllm_head_logprobs_floats": (L, [I, I, I]),
+    "sllm_head_logprobs": (I, [P, P, P, I, I, I, L, C.c_float, I, P, L, P, P, P, P]),
 }
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 MAX_TOP = 32
 MAX_VOCAB = 1 << 30
-CHUNK_LOGITS = 1 << 26         # logits that `linear_logprobs` holds at a time where it writes them
+CHUNK_ROWS = 1 << 15
+CHUNK_LOGITS = 1 << 26         # logits that `linear_logprobs` holds at a time where it writes them,
+CHUNK_FLOATS = 1 << 25         # floats of its workspace where it does not (a sixteenth of the logits' number)
 
 
-def _k():
-    for n, s in _SIGS.items():
-        _lib.EXTRA_KERNEL_SIGNATURES.setdefault(n, s)
-    return _lib.kernels()
+_lib.EXTRA_KERNEL_SIGNATURES.update(_SIGS)
+_k = _lib.kernels
 
 
 class TokenLogprobs(NamedTuple):
@@ -76,29 +79,63 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     log-probabilities of -inf, entropy 0 and no alternatives.  A row with +inf is uniform over those; one with NaN gives NaN and no
     alternatives.  A token below 0 stands for none (0, so that padded places drop out of sums), one from V on gives NaN."""
     if (logits.dim() != 2 or logits.dtype not in _DTYPES or not 1 <= logits.shape[1] <= MAX_VOCAB
-            or (logits.shape[1] > 1 and logits.stride(1) != 1)):
+            or (logits.shape[1] > 1 and logits.stride(1) != 1) or logits.shape[0] >= 2 ** 31):
         raise ValueError(f"logits are bf16, fp16 or fp32 [rows, vocabulary] with contiguous rows of at most {MAX_VOCAB}")
     if not 0 <= top <= MAX_TOP:
         raise ValueError(f"top lies between 0 and {MAX_TOP}")
     _check_tokens(tokens, logits.shape[0], logits.device)
     if _lib.on_cpu(logits):
         return _cpu(logits, tokens, top)
-    from .core import _on, _p, _stream
     r, v = logits.shape
     dev = logits.device
     tokens = tokens.contiguous()
-    lp = torch.empty(tokens.shape, dtype=torch.float32, device=dev)
-    entropy = torch.empty(r, dtype=torch.float32, device=dev)
-    ids = torch.empty((r, top), dtype=torch.int32, device=dev) if top else None
-    tlp = torch.empty((r, top), dtype=torch.float32, device=dev) if top else None
+    given = tokens.shape[1] if tokens.dim() == 2 else 1
+    n = r * given
+    out = torch.empty(n + r + 2 * r * top, dtype=torch.float32, device=dev)      # (one allocation: four cost more than a row's kernel)
+    lp = out.as_strided(tokens.shape, (given, 1) if tokens.dim() == 2 else (1,), 0)
+    entropy = out.as_strided((r,), (1,), n)
+    ids = tlp = None
+    if top:
+        tlp = out.as_strided((r, top), (top, 1), n + r)
+        ids = out.view(torch.int32).as_strided((r, top), (top, 1), n + r + r * top)
     if r:
-        with _on(dev):
-            rc = _k().sllm_token_logprobs(_p(logits), logits.stride(0), r, v, _DTYPES[logits.dtype], _p(tokens), int(tokens.dtype == torch.int64),
-                                          tokens.shape[1] if tokens.dim() == 2 else 1, top, _p(lp), _p(entropy), _p(ids), _p(tlp), _stream())
+        at = out.data_ptr()
+        rc = _launch(dev, _k().sllm_token_logprobs, logits.data_ptr(), logits.stride(0), r, v, _DTYPES[logits.dtype], tokens.data_ptr(),
+                     tokens.dtype == torch.int64, given, top, at, at + 4 * n, at + 4 * (n + r + r * top) if top else None,
+                     at + 4 * (n + r) if top else None)
         _lib.check(rc, "token_logprobs")
         if _lib.audit_enabled():
             _lib.record_dispatch("token_logprobs", "logprobs_kernel", rows=r, vocab=v, top=top)
     return TokenLogprobs(lp, entropy, ids, tlp)
+
+
+def _head(x: torch.Tensor, w: torch.Tensor, tokens: torch.Tensor, softcap: float) -> TokenLogprobs:
+    """bf16 rows against a dense matrix on the tensor cores, without logits in memory."""
+    from . import core
+    r, n, dev = x.shape[0], w.shape[0], x.device
+    out = torch.empty((2, r), dtype=torch.float32, device=dev)
+    lp, entropy = out.unbind()
+    if not r:
+        return TokenLogprobs(lp, entropy)
+    if x.stride(1) != 1 or x.stride(0) % 8 or x.stride(0) < x.shape[1] or x.data_ptr() % 16:      # (a TMA copy needs rows of whole 16 bytes)
+        x = x.contiguous().clone() if x.data_ptr() % 16 else x.contiguous()
+    if tokens.dtype == torch.int64:
+        tokens = tokens.clamp(-1, n).to(torch.int32)
+    tokens = tokens.contiguous()
+    bn = core._prompt_tile(min(r, CHUNK_ROWS), n, False)
+    floats = _k().sllm_head_logprobs_floats
+    step = max(256, min(CHUNK_ROWS, CHUNK_FLOATS // int(floats(1, n, bn))) // 256 * 256)
+    ws = torch.empty(int(floats(min(r, step), n, bn)), dtype=torch.float32, device=dev)
+    status = core.workspace(dev).status
+    for lo in range(0, r, step):
+        m = min(step, r - lo)
+        rc = _launch(dev, _k().sllm_head_logprobs, x.data_ptr() + 2 * lo * x.stride(0), w.data_ptr(), tokens.data_ptr() + 4 * lo, m, n, x.shape[1],
+                     x.stride(0) if r > 1 else x.shape[1], softcap, bn, ws.data_ptr(), ws.numel(), lp.data_ptr() + 4 * lo,
+                     entropy.data_ptr() + 4 * lo, status.data_ptr())
+        _lib.check(rc, "head_logprobs")
+        if _lib.audit_enabled():
+            _lib.record_dispatch("linear_logprobs", "head_logprobs_kernel", m=m, n=n, k=x.shape[1], bn=bn)
+    return TokenLogprobs(lp, entropy)
 
 
 def linear_logprobs(x, w, tokens: torch.Tensor, softcap: float = 0.0, top: int = 0) -> TokenLogprobs:
@@ -116,6 +153,9 @@ def linear_logprobs(x, w, tokens: torch.Tensor, softcap: float = 0.0, top: int =
     _check_tokens(tokens, xd.shape[0], xd.device)
     if tokens.dim() != 1:
         raise ValueError("one token per row")
+    if (not top and w.kind == "dense" and not _lib.on_cpu(xd) and xd.dtype == w.w.dtype == torch.bfloat16 and w.in_features % 8 == 0
+            and w.w.is_contiguous() and w.w.data_ptr() % 16 == 0):
+        return _head(xd, w.w, tokens, softcap)
     step = max(1, CHUNK_LOGITS // w.out_features)
     parts = []
     for lo in range(0, xd.shape[0], step):

@@ -7,6 +7,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib
+from .core import _launch
 
 P, I, L = C.c_void_p, C.c_int, C.c_longlong
 _SIGS = {
@@ -14,10 +15,8 @@ _SIGS = {
 }
 
 
-def _k():
-    for n, s in _SIGS.items():
-        _lib.EXTRA_KERNEL_SIGNATURES.setdefault(n, s)
-    return _lib.kernels()
+_lib.EXTRA_KERNEL_SIGNATURES.update(_SIGS)
+_k = _lib.kernels
 
 
 class BatchPlan(NamedTuple):
@@ -72,13 +71,11 @@ def batch_plan(new_lens: torch.Tensor, starts: torch.Tensor, pages: torch.Tensor
         raise ValueError("the table is int32 [requests, max_blocks] with contiguous rows that do not overlap")
     if _lib.on_cpu(new_lens):
         return _cpu(new_lens, starts, pages, rows, max_blocks, page_size, table)
-    from .core import _on, _p, _stream
-    i32 = lambda n: torch.empty(n, dtype=torch.int32, device=dev)
-    i64 = lambda n: torch.empty(n, dtype=torch.int64, device=dev)
-    out = BatchPlan(i32(s + 1), i32(rows), i32(rows), i32(rows), i64(rows), i64(s), table)
-    with _on(dev):
-        rc = _k().sllm_batch_plan(_p(new_lens), _p(starts), _p(pages), pages.numel(), s, rows, max_blocks,
-                                  table.stride(0) if s > 1 else max_blocks, page_size, _p(out.row_off), _p(out.positions), _p(out.seq_index),
-                                  _p(out.kv_lens), _p(out.slots), _p(out.last_rows), _p(table), _stream())
+    # (two allocations: a tensor of its own for each part costs more than the kernel)
+    row_off, positions, seq_index, kv_lens = torch.empty(s + 1 + 3 * rows, dtype=torch.int32, device=dev).split_with_sizes((s + 1, rows, rows, rows))
+    slots, last_rows = torch.empty(rows + s, dtype=torch.int64, device=dev).split_with_sizes((rows, s))
+    rc = _launch(dev, _k().sllm_batch_plan, new_lens.data_ptr(), starts.data_ptr(), pages.data_ptr(), pages.numel(), s, rows, max_blocks,
+                 table.stride(0) if s > 1 else max_blocks, page_size, row_off.data_ptr(), positions.data_ptr(), seq_index.data_ptr(),
+                 kv_lens.data_ptr(), slots.data_ptr(), last_rows.data_ptr(), table.data_ptr())
     _lib.check(rc, "batch_plan")
-    return out
+    return BatchPlan(row_off, positions, seq_index, kv_lens, slots, last_rows, table)
