@@ -11,8 +11,6 @@
 //   warps 4 ..  two groups of four, thread = row, a group per half of the tile's columns
 // A tile's sum over K is taken in chains of kHlChain K blocks with an accumulator of their own, which the epilogue warps add in fp32
 // registers while the next chain is multiplied: tensor memory rounds towards zero, and a chain's error grows with its length.
-// Few rows need no tile of their own: rows beyond the last are filled with zeros, cost no reading, and their products run beside the
-// reading of W.
 #include <cfloat>
 #include "pair_mma.cuh"
 #include "api.h"
@@ -71,6 +69,64 @@ __device__ __forceinline__ float hl_max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
+}
+
+// Sums of some logits of a row.
+struct HlSums {
+  float m, s, w;
+  __device__ __forceinline__ void add(float om, float os, float ow) {      // NaN passes through
+    const float top = fmaxf(m, om);
+    const float t = m == top ? 0.f : fmaxf((m - top) * kHlLog2e, -1000.f), e = hl_exp2(t);
+    const float u = om == top ? 0.f : fmaxf((om - top) * kHlLog2e, -1000.f), f = hl_exp2(u);
+    w = e * fmaf(t, s, w) + f * fmaf(u, os, ow);
+    s = e * s + f * os;
+    m = top;
+  }
+};
+
+// The part of a row that lies in columns n0 .. n0 + width - 1 (nothing with width <= 0): caps the logits, leaves the given token's behind and
+// sums up.  All lanes of a warp take part.
+template <int kCols>
+__device__ __forceinline__ HlSums hl_reduce(const HlParams& p, float (&z)[kCols], int token, int row, int n0, int width) {
+  if (p.cap > 0.f) {
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) z[c] = p.cap * tanhf(z[c] * p.inv_cap);
+  }
+  const int at = token - n0;
+  const bool here = token >= n0 && at < width;
+  if (__any_sync(0xffffffffu, here)) {
+    float x = 0.f;
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) x = at == c ? z[c] : x;
+    if (here) p.given[row] = x;
+  }
+  if (width < kCols) {
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) z[c] = c < width ? z[c] : -INFINITY;
+  }
+  float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int c = 0; c < kCols; c += 4)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m4[i] = fmaxf(m4[i], z[c + i]);
+  const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+  float s0 = 0.f, s1 = 0.f, w0 = 0.f, w1 = 0.f;
+  if (m < INFINITY) {
+    const float ref = m > -INFINITY ? m : 0.f;             // (nothing but -inf: every term is 2^-1000)
+#pragma unroll
+    for (int c = 0; c < kCols; c += 2) {
+      const float t0 = hl_max_nan((z[c] - ref) * kHlLog2e, -1000.f), t1 = hl_max_nan((z[c + 1] - ref) * kHlLog2e, -1000.f);
+      const float e0 = hl_exp2(t0), e1 = hl_exp2(t1);
+      s0 += e0;
+      s1 += e1;
+      w0 = fmaf(e0, t0, w0);
+      w1 = fmaf(e1, t1, w1);
+    }
+  } else {                                                 // uniform over +inf
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) s0 += z[c] != z[c] ? z[c] : z[c] == INFINITY ? 1.f : 0.f;
+  }
+  return {m, s0 + s1, w0 + w1};
 }
 
 template <int BN>
@@ -200,43 +256,8 @@ head_logprobs_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
         if (lane == 0) mbar_arrive_remote(empty_addr + 8 * (acc % S::kAcc));
       }
       if (!ok) break;
-      if (p.cap > 0.f) {
-#pragma unroll
-        for (int c = 0; c < S::kCols; ++c) z[c] = p.cap * tanhf(z[c] * p.inv_cap);
-      }
-      if (__any_sync(0xffffffffu, token >= n0 && token < n0 + S::kCols)) {
-        float x = 0.f;
-#pragma unroll
-        for (int c = 0; c < S::kCols; ++c) x = token - n0 == c ? z[c] : x;
-        if (token >= n0 && token < min(n0 + S::kCols, p.n)) p.given[row] = x;
-      }
-      if (n0 + S::kCols > p.n) {                           // tokens beyond the last
-#pragma unroll
-        for (int c = 0; c < S::kCols; ++c) z[c] = n0 + c < p.n ? z[c] : -INFINITY;
-      }
-      float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int c = 0; c < S::kCols; c += 4)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) m4[i] = fmaxf(m4[i], z[c + i]);
-      const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-      float s0 = 0.f, s1 = 0.f, w0 = 0.f, w1 = 0.f;
-      if (m < INFINITY) {
-        const float ref = m > -INFINITY ? m : 0.f;         // (nothing but -inf: every term is 2^-1000)
-#pragma unroll
-        for (int c = 0; c < S::kCols; c += 2) {
-          const float t0 = hl_max_nan((z[c] - ref) * kHlLog2e, -1000.f), t1 = hl_max_nan((z[c + 1] - ref) * kHlLog2e, -1000.f);
-          const float e0 = hl_exp2(t0), e1 = hl_exp2(t1);
-          s0 += e0;
-          s1 += e1;
-          w0 = fmaf(e0, t0, w0);
-          w1 = fmaf(e1, t1, w1);
-        }
-      } else {                                             // uniform over +inf
-#pragma unroll
-        for (int c = 0; c < S::kCols; ++c) s0 += z[c] != z[c] ? z[c] : z[c] == INFINITY ? 1.f : 0.f;
-      }
-      if (row < p.m) p.part[static_cast<size_t>(2 * tn + grp) * p.m + row] = make_float4(m, s0 + s1, w0 + w1, 0.f);
+      const HlSums part = hl_reduce<S::kCols>(p, z, token, row, n0, min(p.n - n0, S::kCols));
+      if (row < p.m) p.part[static_cast<size_t>(2 * tn + grp) * p.m + row] = make_float4(part.m, part.s, part.w, 0.f);
     }
   }
   tc_fence_before();
@@ -248,19 +269,156 @@ head_logprobs_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
   }
 }
 
+// Up to 128 rows, where the reading of W is what there is to do: one CTA per SM with an equal share of W's rows (kHfBox of them to
+// a copy), so that no CTA reads longer than the others, in tiles of up to 256.  One tensor-core row is one row of X; a CTA's tiles
+// belong to the same rows, whose sums stay in registers until the end.
+constexpr int kHfBox = 16, kHfTile = 256, kHfStages = 4, kHfCols = kHfTile / 2;
+constexpr int kHfABytes = kHlRows * 128, kHfStage = kHfABytes + kHfTile * 128;
+
+__global__ void __launch_bounds__(kHlThreads, 1)
+head_few_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w, const HlParams p, int share, int x_rows) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  HlShared* sh = reinterpret_cast<HlShared*>(smem + kHfStages * kHfStage);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int first_n = blockIdx.x * share, last_n = min(first_n + share, p.n);      // the CTA's columns
+  volatile int* abort_flag = &sh->abort_flag;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kHfStages; ++s) {
+      mbar_init(&sh->full[s], 1);
+      mbar_init(&sh->empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&sh->acc_full[b], 1);
+      mbar_init(&sh->acc_empty[b], 8);
+    }
+    sh->abort_flag = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&tm_x);
+    tma_prefetch_desc(&tm_w);
+  }
+  if (warp == 1) {
+    tmem_alloc(&sh->tmem_base, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = sh->tmem_base;
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == 0) {
+      if (elect_one()) {
+        pdl_wait();
+        const int turn = static_cast<int>(blockIdx.x * static_cast<long long>(p.num_kb) / gridDim.x);
+        int it = 0;                                        // K blocks over all tiles
+        bool ok = true;
+        for (int n0 = first_n; ok && n0 < last_n; n0 += kHfTile) {
+          const int boxes = (min(kHfTile, last_n - n0) + kHfBox - 1) / kHfBox;
+          for (int kb = 0; kb < p.num_kb; ++kb, ++it) {
+            const int s = it % kHfStages;
+            if (it >= kHfStages && !mbar_wait(&sh->empty[s], ((it / kHfStages) & 1) ^ 1, abort_flag, p.status, SLLM_DEV_TIMEOUT_SMEM_EMPTY)) {
+              ok = false;
+              break;
+            }
+            uint8_t* dst = smem + s * kHfStage;
+            mbar_expect_tx(&sh->full[s], x_rows * 128 + boxes * kHfBox * 128);
+            int k0 = kb + turn;
+            k0 = (k0 < p.num_kb ? k0 : k0 - p.num_kb) * 64;
+            for (int b = 0; b < boxes; ++b) tma_load_2d(dst + kHfABytes + b * kHfBox * 128, &tm_w, &sh->full[s], k0, n0 + b * kHfBox);
+            tma_load_2d(dst, &tm_x, &sh->full[s], k0, 0);
+          }
+        }
+        pdl_trigger();
+        // every copy has landed before the CTA may leave (at once unless something gave up): a stage's last fill
+        int dummy = 0;
+        for (int j = max(0, it - kHfStages); j < it; ++j)
+          mbar_wait(&sh->full[j % kHfStages], (j / kHfStages) & 1, &dummy, p.status, SLLM_DEV_TIMEOUT_DRAIN, 200000000LL);
+      }
+      __syncwarp();
+    } else if (warp == 1) {
+      int it = 0, acc = 0;                                 // acc: accumulators handed over so far
+      bool ok = true;
+      for (int n0 = first_n; ok && n0 < last_n; n0 += kHfTile) {
+        const int boxes = (min(kHfTile, last_n - n0) + kHfBox - 1) / kHfBox;
+        const uint32_t idesc = make_idesc(kFmtBf16, 128, boxes * kHfBox);
+        for (int kb = 0; kb < p.num_kb; ++kb, ++it) {
+          const int s = it % kHfStages, buf = acc & 1;
+          const bool first = kb % kHlChain == 0, last = kb % kHlChain == kHlChain - 1 || kb == p.num_kb - 1;
+          ok = mbar_wait(&sh->full[s], (it / kHfStages) & 1, abort_flag, p.status, SLLM_DEV_TIMEOUT_TMA_FULL);
+          if (ok && first) ok = mbar_wait(&sh->acc_empty[buf], ((acc / 2) & 1) ^ 1, abort_flag, p.status, SLLM_DEV_TIMEOUT_TMEM_EMPTY);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t a_addr = smem_u32(smem + s * kHfStage);
+          const uint64_t ad = make_smem_desc_sw128(a_addr), bd = make_smem_desc_sw128(a_addr + kHfABytes);
+          if (elect_one()) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) umma_f16(tmem_base + buf * kHfTile, ad + 2 * k, bd + 2 * k, idesc, k > 0 || !first);
+            tc_commit(&sh->empty[s]);
+            if (last) tc_commit(&sh->acc_full[buf]);
+          }
+          __syncwarp();
+          acc += last;
+        }
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    pdl_wait();
+    const int q = warp & 3, grp = (warp - 4) >> 2, row = q * 32 + lane;
+    const bool idle = q * 32 >= p.m;                       // a warp without rows only hands the accumulators back
+    const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + grp * kHfCols;
+    const int token = row < p.m ? p.tokens[row] : -1;
+    HlSums all = {-INFINITY, 0.f, 0.f};
+    int acc = 0;
+    bool ok = true;
+    for (int n0 = first_n; ok && n0 < last_n; n0 += kHfTile) {
+      const int mine = n0 + grp * kHfCols, width = min(last_n - mine, kHfCols);
+      const bool skip = idle || width <= 0;
+      float z[kHfCols];
+#pragma unroll
+      for (int c = 0; c < kHfCols; ++c) z[c] = 0.f;
+      for (int chain = 0; chain < p.chains; ++chain, ++acc) {
+        ok = mbar_wait(&sh->acc_full[acc & 1], (acc / 2) & 1, abort_flag, p.status, SLLM_DEV_TIMEOUT_TMEM_FULL);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        if (!skip) {
+#pragma unroll
+          for (int c = 0; c < kHfCols / 32; ++c) {
+            if (c * 32 >= width) break;                    // (columns of no product are not read)
+            uint32_t r[32];
+            tmem_ld32(lane_addr + (acc & 1) * kHfTile + c * 32, r);
+            tmem_wait_regs(r);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) z[c * 32 + j] += __uint_as_float(r[j]);
+          }
+        }
+        tc_fence_before();                                 // all of it is in registers
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->acc_empty[acc & 1]);
+      }
+      if (!ok) break;
+      if (!skip) {
+        const HlSums part = hl_reduce<kHfCols>(p, z, token, row, mine, width);
+        all.add(part.m, part.s, part.w);
+      }
+    }
+    if (row < p.m) p.part[static_cast<size_t>(2 * blockIdx.x + grp) * p.m + row] = make_float4(all.m, all.s, all.w, 0.f);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
 // The parts of a row: eight rows per CTA, so that a line of parts is read as a whole, 128 threads for each.
 constexpr int kHlJoinRows = 8, kHlJoinThreads = 1024;
-struct HlSums {
-  float m, s, w;
-  __device__ __forceinline__ void add(float om, float os, float ow) {      // NaN passes through
-    const float top = fmaxf(m, om);
-    const float t = m == top ? 0.f : fmaxf((m - top) * kHlLog2e, -1000.f), e = hl_exp2(t);
-    const float u = om == top ? 0.f : fmaxf((om - top) * kHlLog2e, -1000.f), f = hl_exp2(u);
-    w = e * fmaf(t, s, w) + f * fmaf(u, os, ow);
-    s = e * s + f * os;
-    m = top;
-  }
-};
 __global__ void __launch_bounds__(kHlJoinThreads)
 head_join_kernel(const float4* __restrict__ part, const float* __restrict__ given, const int* __restrict__ tokens, int m, int n, int parts,
                  float* __restrict__ logprob, float* __restrict__ entropy) {
@@ -305,6 +463,13 @@ head_join_kernel(const float4* __restrict__ part, const float* __restrict__ give
   entropy[row] = bad ? nan : all.m > -INFINITY ? (log_s - all.w / all.s) * kHlLn2 : 0.f;
 }
 
+static int head_join(const HlParams& p, int parts, float* logprob, float* entropy, cudaStream_t st) {
+  return launch_kernel(head_join_kernel, dim3((p.m + kHlJoinRows - 1) / kHlJoinRows), dim3(kHlJoinThreads), 0, st, 1u, p.part, p.given,
+                       p.tokens, p.m, p.n, parts, logprob, entropy) == cudaSuccess
+             ? SLLM_OK
+             : SLLM_ERR_CUDA;
+}
+
 template <int BN>
 static int head_logprobs_go(const void* x, const void* w, int k, long long ldx, HlParams& p, float* logprob, float* entropy, cudaStream_t st) {
   using S = HlShape<BN>;
@@ -322,29 +487,57 @@ static int head_logprobs_go(const void* x, const void* w, int k, long long ldx, 
   const int pairs = tiles < 74 ? static_cast<int>(tiles) : 74;
   if (launch_kernel_cluster(head_logprobs_kernel<BN>, dim3(2 * pairs), dim3(kHlThreads), smem, st, 2u, 1u, tx, tw, p) != cudaSuccess)
     return SLLM_ERR_CUDA;
-  return launch_kernel(head_join_kernel, dim3((p.m + kHlJoinRows - 1) / kHlJoinRows), dim3(kHlJoinThreads), 0, st, 1u, p.part, p.given,
-                       p.tokens, p.m, p.n, 2 * p.tiles_n, logprob, entropy) == cudaSuccess
-             ? SLLM_OK
-             : SLLM_ERR_CUDA;
+  return head_join(p, 2 * p.tiles_n, logprob, entropy, st);
+}
+
+// CTAs of the kernel for few rows, and the columns of each.
+static void head_few_shape(int n, int& ctas, int& share) {
+  share = ((n + 147) / 148 + kHfBox - 1) / kHfBox * kHfBox;
+  ctas = (n + share - 1) / share;
+}
+
+static int head_few_go(const void* x, const void* w, int k, long long ldx, HlParams& p, float* logprob, float* entropy, cudaStream_t st) {
+  CUtensorMap tx, tw;
+  int x_rows = 8;                           // rows of X that are copied: what lies behind them in shared memory reaches no row that counts
+  while (x_rows < p.m) x_rows *= 2;
+  int rc = cached_kmajor_tmap(&tx, x, 2, p.m, k, ldx * 2, x_rows);
+  if (rc == SLLM_OK) rc = cached_kmajor_tmap(&tw, w, 2, p.n, k, static_cast<long long>(k) * 2, kHfBox);
+  if (rc != SLLM_OK) return rc;
+  int ctas, share;
+  head_few_shape(p.n, ctas, share);
+  if ((share / kHfTile + 1LL) * p.num_kb > 0x7fffffffLL) return SLLM_ERR_LIMIT;
+  const size_t smem = kHfStages * kHfStage + sizeof(HlShared) + 1024;
+  if (cudaFuncSetAttribute(head_few_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess)
+    return SLLM_ERR_CUDA;
+  if (launch_kernel(head_few_kernel, dim3(ctas), dim3(kHlThreads), smem, st, 1u, tx, tw, p, share, x_rows) != cudaSuccess) return SLLM_ERR_CUDA;
+  return head_join(p, 2 * ctas, logprob, entropy, st);
 }
 
 }  // namespace sllm
 
 using namespace sllm;
 
+// Parts of a row: two per tile of bn columns (128 or 256, of CTA pairs), or with bn = 0 two per CTA of the kernel for up to 128 rows.
+static long long head_parts(int n, int bn) {
+  if (bn) return 2 * ((n + bn - 1LL) / bn);
+  int ctas, share;
+  head_few_shape(n, ctas, share);
+  return 2LL * ctas;
+}
+
 // Floats of workspace that m rows take with n tokens.
 SLLM_EXPORT long long sllm_head_logprobs_floats(int m, int n, int bn) {
-  if (m <= 0 || n <= 0 || (bn != 128 && bn != 256)) return 0;
-  return static_cast<long long>(m) * (8LL * ((n + bn - 1LL) / bn) + 1);
+  if (m <= 0 || n <= 0 || n > (1 << 30) || (bn != 0 && bn != 128 && bn != 256)) return 0;
+  return m * (4 * head_parts(n, bn) + 1);
 }
 
 // x [m, k] bf16 (row stride ldx elements), w [n, k] bf16 contiguous, tokens [m]; logprob and entropy [m].  cap > 0: soft cap.  bn: columns
-// of a pair's tile, 128 or 256.  k a multiple of 8, rows of x multiples of 16 bytes.
+// of a CTA pair's tile, 128 or 256; 0: the kernel for up to 128 rows.  k a multiple of 8, rows of x multiples of 16 bytes.
 SLLM_EXPORT int sllm_head_logprobs(const void* x, const void* w, const int* tokens, int m, int n, int k, long long ldx, float cap, int bn,
                                    float* ws, long long ws_floats, float* logprob, float* entropy, int* status, void* stream) {
   if (!x || !w || !tokens || !ws || !logprob || !entropy || m <= 0 || n <= 0 || k <= 0 || ldx < k || !(cap >= 0.f && cap < INFINITY))
     return SLLM_ERR_INVALID_ARGUMENT;
-  if (bn != 128 && bn != 256) return SLLM_ERR_INVALID_ARGUMENT;
+  if ((bn != 0 && bn != 128 && bn != 256) || (bn == 0 && m > kHlRows)) return SLLM_ERR_INVALID_ARGUMENT;
   if (m > (1 << 24) || n > (1 << 30) || k > (1 << 24)) return SLLM_ERR_LIMIT;
   if ((k & 7) || (ldx & 7) || ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(ws)) & 15))
     return SLLM_ERR_ALIGNMENT;
@@ -353,8 +546,9 @@ SLLM_EXPORT int sllm_head_logprobs(const void* x, const void* w, const int* toke
   p.m = m; p.n = n; p.num_kb = (k + 63) / 64; p.chains = (p.num_kb + kHlChain - 1) / kHlChain;
   p.cap = cap; p.inv_cap = cap > 0.f ? 1.f / cap : 0.f;
   p.tokens = tokens; p.part = reinterpret_cast<float4*>(ws);
-  p.given = ws + static_cast<long long>(m) * 8 * ((n + bn - 1) / bn);
+  p.given = ws + 4 * head_parts(n, bn) * m;
   p.status = status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (bn == 0) return head_few_go(x, w, k, ldx, p, logprob, entropy, st);
   return bn == 256 ? head_logprobs_go<256>(x, w, k, ldx, p, logprob, entropy, st) : head_logprobs_go<128>(x, w, k, ldx, p, logprob, entropy, st);
 }

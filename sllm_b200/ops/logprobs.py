@@ -20,6 +20,7 @@ _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 MAX_TOP = 32
 MAX_VOCAB = 1 << 30
 CHUNK_ROWS = 1 << 15
+FEW_ROWS = 128                 # up to here a row's tile is shared by no CTA pair (csrc/head_logprobs.cu)
 CHUNK_LOGITS = 1 << 26         # logits that `linear_logprobs` holds at a time where it writes them,
 CHUNK_FLOATS = 1 << 25         # floats of its workspace where it does not (a sixteenth of the logits' number)
 
@@ -122,7 +123,7 @@ def _head(x: torch.Tensor, w: torch.Tensor, tokens: torch.Tensor, softcap: float
     if tokens.dtype == torch.int64:
         tokens = tokens.clamp(-1, n).to(torch.int32)
     tokens = tokens.contiguous()
-    bn = core._prompt_tile(min(r, CHUNK_ROWS), n, False)
+    bn = 0 if r <= FEW_ROWS else core._prompt_tile(min(r, CHUNK_ROWS), n, False)
     floats = _k().sllm_head_logprobs_floats
     step = max(256, min(CHUNK_ROWS, CHUNK_FLOATS // int(floats(1, n, bn))) // 256 * 256)
     ws = torch.empty(int(floats(min(r, step), n, bn)), dtype=torch.float32, device=dev)

@@ -31,7 +31,7 @@ def oracle(z, ids, top):
             h = -float((p[p > 0] * logp[p > 0]).sum())
         lps.append([0.0 if t < 0 else NAN if t >= v else float(logp[t]) for t in given])
         hs.append(h)
-        order = [] if math.isnan(h) else [i for i in sorted(range(v), key=lambda i: (-float(row[i]), i))[:top] if row[i] != -INF]
+        order = [] if math.isnan(h) or not top else [i for i in torch.argsort(row, descending=True, stable=True)[:top].tolist() if row[i] != -INF]
         tids.append(order + [-1] * (top - len(order)))
         tlps.append([float(logp[i]) for i in order] + [NAN if math.isnan(h) else -INF] * (top - len(order)))
     t = lambda x: torch.tensor(x, dtype=torch.float64)
@@ -157,6 +157,23 @@ def test_the_launcher_refuses():
         assert f(*a) == code, (at, value)
 
 
+def test_the_head_launcher_refuses():
+    if not _lib.kernels_available():
+        pytest.skip("the kernel library is not built")
+    f, floats = LP._k().sllm_head_logprobs, LP._k().sllm_head_logprobs_floats
+    for bn in (0, 128, 256):
+        assert floats(0, 8, bn) == 0 and floats(5, 70000, bn) % 5 == 0
+    assert floats(5, 8, 64) == 0 and floats(5, (1 << 30) + 1, 0) == 0
+    ok = [256, 256, 256, 100, 1000, 64, 64, 0.0, 256, 256, 1 << 20, 256, 256, 256, None]
+    for at, value, code in ((0, None, 1), (1, None, 1), (2, None, 1), (3, 0, 1), (4, 0, 1), (5, 0, 1), (6, 63, 1), (7, -1.0, 1), (7, NAN, 1), (7, INF, 1),
+                            (8, 64, 1), (9, None, 1), (11, None, 1), (12, None, 1), (3, (1 << 24) + 1, 7), (4, (1 << 30) + 1, 7), (6, 68, 3), (0, 264, 3),
+                            (1, 264, 3), (9, 264, 3), (10, floats(100, 1000, 256) - 1, 4)):
+        a = list(ok)
+        a[at] = value
+        assert f(*a) == code, (at, value)
+    assert f(*(ok[:3] + [129] + ok[4:8] + [0] + ok[9:])) == 1          # more rows than the kernel for few takes
+
+
 # ------------------------------------------------------------------------------------------ kernels
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
@@ -257,7 +274,7 @@ def head_check(x, w, ids, cap, got, extra=0):
 
 
 HEADS = [(1, 8, 1), (1, 64, 300), (3, 72, 1000), (16, 512, 2048), (17, 128, 777), (128, 64, 257), (129, 200, 1025), (300, 1024, 5000), (513, 8, 40),
-         (40, 4096, 3001)]
+         (40, 4096, 3001), (5, 64, 100003), (128, 40, 76001), (600, 64, 20000), (257, 1536, 9001)]
 
 
 @pytest.mark.gpu
@@ -288,3 +305,80 @@ def test_head_with_alternatives_and_quantised_weights():
         got = ops.linear_logprobs(rows_, fp8, ids, top=4)
         want = ops.token_logprobs(ops.linear(rows_, fp8), ids, 4)
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("r", [7, 200])
+def test_head_at_the_edges(r):
+    """Tokens of no row and none, int64 tokens, rows of a wider matrix, off 16 bytes and in reverse order, infinities and NaN."""
+    x, w, ids = head_case(r, 64, 999, 5)
+    lw = ops.LinearWeight("dense", w)
+    want = ops.linear_logprobs(x, lw, ids)
+    odd = ids.long()
+    odd[0], odd[1], odd[2] = -1, 999, 1 << 40
+    got = ops.linear_logprobs(x, lw, odd)
+    assert float(got.logprob[0]) == 0.0 and bool(torch.isnan(got.logprob[1:3]).all()) and torch.equal(got.logprob[3:], want.logprob[3:])
+    assert torch.equal(got.entropy, want.entropy)
+    wide = torch.zeros((r, 80), dtype=torch.bfloat16, device=DEV)
+    for view in (wide[:, 8:72], wide[:, 3:67], torch.zeros((r, 64 + 1), dtype=torch.bfloat16, device=DEV)[:, 1:]):
+        view.copy_(x)
+        got = ops.linear_logprobs(view, lw, ids)
+        assert torch.equal(got.logprob, want.logprob) and torch.equal(got.entropy, want.entropy)
+    got = ops.linear_logprobs(x.t().contiguous().t(), lw, ids)
+    assert torch.equal(got.logprob, want.logprob)
+    x = x.clone()
+    x[0, 0], x[1, 5], x[2] = INF, NAN, 0.0
+    w2 = w.clone()
+    w2[:, 0] = w2[:, 0].abs()                              # row 0: every logit +inf
+    z = x.double() @ w2.double().t()
+    got = ops.linear_logprobs(x, ops.LinearWeight("dense", w2), ids)
+    lp, h, _, _ = oracle(z[:3], ids[:3], 0)
+    same(got.logprob[:3], lp, 1e-5)                        # logarithms of 999, rounded to 2^-24 twice, and sums of 999 equal terms
+    same(got.entropy[:3], h, 1e-5)
+    assert bool(torch.isfinite(got.logprob[3:]).all())     # a row's values reach no other row
+
+
+@pytest.mark.gpu
+def test_head_of_nothing_but_minus_infinity():
+    x = torch.ones((2, 8), dtype=torch.bfloat16, device=DEV)
+    w = torch.full((300, 8), -INF, dtype=torch.bfloat16, device=DEV)
+    for rows_ in (x, x.repeat(100, 1)):
+        got = ops.linear_logprobs(rows_, ops.LinearWeight("dense", w), torch.zeros(rows_.shape[0], dtype=torch.int32, device=DEV))
+        assert bool((got.logprob == -INF).all()) and bool((got.entropy == 0).all())
+        w2 = w.clone()
+        w2[::3] = 0.25                                     # 100 tokens of one logit each
+        got = ops.linear_logprobs(rows_, ops.LinearWeight("dense", w2), torch.ones(rows_.shape[0], dtype=torch.int32, device=DEV))
+        assert bool((got.logprob == -INF).all())
+        same(got.entropy, torch.full((rows_.shape[0],), math.log(100.0), dtype=torch.float64), 1e-5)
+
+
+@pytest.mark.gpu
+def test_head_in_chunks_streams_and_graphs(monkeypatch):
+    x, w, ids = head_case(700, 72, 1111, 6)
+    lw = ops.LinearWeight("dense", w)
+    want = ops.linear_logprobs(x, lw, ids)
+    monkeypatch.setattr(LP, "CHUNK_ROWS", 256)
+    got = ops.linear_logprobs(x, lw, ids)
+    monkeypatch.undo()
+    assert torch.equal(got.logprob, want.logprob) and torch.equal(got.entropy, want.entropy)
+    few = x[:9].clone()
+    first = ops.linear_logprobs(few, lw, ids[:9])
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        a, b = ops.linear_logprobs(few, lw, ids[:9]), ops.linear_logprobs(x, lw, ids)
+    c, d = ops.linear_logprobs(x, lw, ids), ops.linear_logprobs(few, lw, ids[:9])
+    torch.cuda.synchronize()
+    for got, whole in ((a, first), (b, want), (c, want), (d, first)):
+        assert torch.equal(got.logprob, whole.logprob) and torch.equal(got.entropy, whole.entropy)
+    g1, g2 = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g1):
+        p = ops.linear_logprobs(few, lw, ids[:9])
+    with torch.cuda.graph(g2):
+        q = ops.linear_logprobs(x, lw, ids)
+    few.copy_(x[100:109])
+    for g in (g1, g2, g1):
+        g.replay()
+    again = ops.linear_logprobs(x[100:109], lw, ids[:9])
+    assert torch.equal(p.logprob, again.logprob) and torch.equal(q.logprob, want.logprob) and torch.equal(q.entropy, want.entropy)
+    assert ops.device_status(x.device) == 0
