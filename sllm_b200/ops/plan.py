@@ -17,6 +17,8 @@ _SIGS = {
 
 _lib.EXTRA_KERNEL_SIGNATURES.update(_SIGS)
 _k = _lib.kernels
+MAX_REQUESTS = 16384           # whose running sums fit in shared memory
+MAX_COUNT = 2 ** 31 - 4096
 
 
 class BatchPlan(NamedTuple):
@@ -55,25 +57,30 @@ def batch_plan(new_lens: torch.Tensor, starts: torch.Tensor, pages: torch.Tensor
     ``pages`` (int32): the requests' pages one after another, ceil((starts + new_lens) / page_size) of each.  ``rows``: rows of the
     batch, the sum of new_lens or more (a captured step's padding).  ``table`` (int32 [S, max_blocks], any row stride) receives
     the block table in place of a new tensor.  A length below 0 counts as 0; entries whose page lies beyond the list read page 0, and
-    a table narrower than a request holds its first pages.  Positions stay below 2^31."""
+    a table narrower than a request holds its first pages.  Positions stay below 2^31, requests at 16384 or less."""
     for t in (new_lens, starts, pages):
         if t.dtype != torch.int32 or t.dim() != 1 or t.device != new_lens.device or not t.is_contiguous():
             raise ValueError("lengths, starts and pages are contiguous int32 vectors on one device")
     s, dev = new_lens.numel(), new_lens.device
     if starts.numel() != s:
         raise ValueError("one start per length")
-    if not 0 <= rows < 2 ** 31 or not 0 <= max_blocks < 2 ** 31 or not 1 <= page_size < 2 ** 31 or s >= 2 ** 31:
-        raise ValueError("rows, max_blocks and page_size are counts below 2^31")
-    if table is None:
-        table = torch.empty((s, max_blocks), dtype=torch.int32, device=dev)
-    elif (table.dtype != torch.int32 or table.shape != (s, max_blocks) or table.device != dev or (max_blocks > 1 and table.stride(1) != 1)
-          or (s > 1 and table.stride(0) < max_blocks)):
+    if s > MAX_REQUESTS:
+        raise ValueError(f"at most {MAX_REQUESTS} requests")
+    if not 0 <= rows <= MAX_COUNT or not 0 <= max_blocks <= MAX_COUNT or not 1 <= page_size < 2 ** 31 or pages.numel() >= 2 ** 31:
+        raise ValueError("rows, max_blocks, page_size and pages are counts below 2^31")
+    if table is not None and (table.dtype != torch.int32 or table.shape != (s, max_blocks) or table.device != dev
+                              or (max_blocks > 1 and table.stride(1) != 1) or (s > 1 and table.stride(0) < max_blocks)):
         raise ValueError("the table is int32 [requests, max_blocks] with contiguous rows that do not overlap")
     if _lib.on_cpu(new_lens):
-        return _cpu(new_lens, starts, pages, rows, max_blocks, page_size, table)
-    # (two allocations: a tensor of its own for each part costs more than the kernel)
-    row_off, positions, seq_index, kv_lens = torch.empty(s + 1 + 3 * rows, dtype=torch.int32, device=dev).split_with_sizes((s + 1, rows, rows, rows))
-    slots, last_rows = torch.empty(rows + s, dtype=torch.int64, device=dev).split_with_sizes((rows, s))
+        return _cpu(new_lens, starts, pages, rows, max_blocks, page_size,
+                    torch.empty((s, max_blocks), dtype=torch.int32) if table is None else table)
+    # (one allocation: a tensor of its own for each part costs more than the kernel)
+    cells = 0 if table is not None else s * max_blocks
+    n32 = cells + s + 1 + 3 * rows
+    rest, slots, last_rows = torch.empty(n32 // 2 + 1 + rows + s, dtype=torch.int64, device=dev).split_with_sizes((n32 // 2 + 1, rows, s))
+    own, row_off, positions, seq_index, kv_lens, _ = rest.view(torch.int32).split_with_sizes((cells, s + 1, rows, rows, rows, 2 - n32 % 2))
+    if table is None:
+        table = own.view(s, max_blocks)
     rc = _launch(dev, _k().sllm_batch_plan, new_lens.data_ptr(), starts.data_ptr(), pages.data_ptr(), pages.numel(), s, rows, max_blocks,
                  table.stride(0) if s > 1 else max_blocks, page_size, row_off.data_ptr(), positions.data_ptr(), seq_index.data_ptr(),
                  kv_lens.data_ptr(), slots.data_ptr(), last_rows.data_ptr(), table.data_ptr())

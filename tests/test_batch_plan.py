@@ -41,7 +41,8 @@ CASES = [case([1], [0], 16) + (0, 1, 16), case([1], [15], 16) + (0, 1, 16), case
          case(lens(300, 40, 2), lens(300, 70, 3), 16) + (11, 7, 16), case(lens(1000, 3, 4), lens(1000, 20, 5), 1) + (1, 24, 1),
          case(lens(2100, 2, 6), lens(2100, 5, 7), 4) + (0, 2, 4), case(lens(7, 900, 8), lens(7, 900, 9), 48, short=9) + (0, 33, 48),
          case([4, -3, 2], [-8, 20, 3], 16) + (1, 3, 16), case([0, 0, 0], [0, 0, 0], 16) + (4, 2, 16), case([20, 3], [0, 0], 16) + (-9, 3, 16),
-         case(lens(9, 4000, 10), [0] * 9, 16) + (0, 0, 16)]
+         case(lens(9, 4000, 10), [0] * 9, 16) + (0, 0, 16), case([1] * 40 + [30000] + [2] * 40, [17] * 81, 16) + (600, 1900, 16),
+         case(lens(16384, 2, 11), lens(16384, 9, 12), 4) + (7, 4, 4), case([9, 1, 600], [0, 4095, 70000], 16) + (0, 5000, 16)]
 
 
 def same(got, want):
@@ -64,7 +65,7 @@ def test_refusals():
     good = dict(new_lens=i(2, 3), starts=i(0, 0), pages=i(0, 1), rows=5, max_blocks=2, page_size=16)
     ops.batch_plan(**good)
     for bad in (dict(new_lens=i(2, 3).long()), dict(starts=i(0)), dict(pages=i(0, 1).float()), dict(new_lens=i(2, 3).view(1, 2)), dict(rows=-1),
-                dict(rows=2 ** 31), dict(max_blocks=-1), dict(page_size=0), dict(starts=torch.zeros(4, dtype=torch.int32)[::2]),
+                dict(rows=2 ** 31), dict(new_lens=torch.zeros(20000, dtype=torch.int32), starts=torch.zeros(20000, dtype=torch.int32)), dict(max_blocks=-1), dict(page_size=0), dict(starts=torch.zeros(4, dtype=torch.int32)[::2]),
                 dict(table=torch.zeros((2, 3), dtype=torch.int32)), dict(table=torch.zeros((2, 2))), dict(table=torch.zeros((2, 2), dtype=torch.int32).t()),
                 dict(table=torch.zeros((1, 2), dtype=torch.int32).expand(2, 2))):
         with pytest.raises(ValueError):
@@ -76,6 +77,7 @@ def test_the_launcher_refuses():
         pytest.skip("the kernel library is not built")
     f = PL._k().sllm_batch_plan
     ok = [256, 256, 256, 4, 2, 5, 2, 2, 16, 256, 256, 256, 256, 256, 256, 256, None]
+    assert f(*(ok[:4] + [16385] + ok[5:])) == 7 and f(*(ok[:5] + [2 ** 31 - 1] + ok[6:])) == 7 and f(*(ok[:3] + [2 ** 31] + ok[4:])) == 7
     for at, value in ((0, None), (1, None), (2, None), (3, -1), (4, -1), (5, -1), (6, -1), (7, 1), (8, 0), (9, None), (10, None), (13, None),
                       (14, None), (15, None)):
         a = list(ok)
