@@ -43,6 +43,7 @@ class PagePool:
     def __init__(self, num_pages: int, page_size: int = 16):
         self._lib = _lib.host()
         self._lib.sllm_kv_seq_length.restype = C.c_longlong
+        self._lib.sllm_kv_list_pages.restype = C.c_longlong
         self._lib.sllm_kv_seq_reserve.argtypes = [C.c_int, C.c_int, C.c_longlong]
         self._lib.sllm_kv_seq_commit.argtypes = [C.c_int, C.c_int, C.c_longlong]
         self._lib.sllm_kv_seq_truncate.argtypes = [C.c_int, C.c_int, C.c_longlong]
@@ -126,6 +127,20 @@ class PagePool:
 
     def inject_alloc_failure(self, after_calls: int) -> None:
         self._lib.sllm_kv_pool_inject_alloc_failure(self.h, after_calls)
+
+    def list_pages(self, seqs: list, lengths: list, out=None):
+        """Pages that hold the first lengths[i] tokens of every sequence, one sequence after another: an int32 array, a part of
+        ``out`` (a contiguous int32 CPU tensor) where one is given."""
+        counts = [(n + self.page_size - 1) // self.page_size for n in lengths]
+        total = sum(counts)
+        if out is None:
+            out = torch.empty(total, dtype=torch.int32)
+        arr = (C.c_int * len(seqs))(*seqs)
+        n = self._lib.sllm_kv_list_pages(self.h, arr, (C.c_int * len(seqs))(*counts), len(seqs), C.c_void_p(out.data_ptr()),
+                                         C.c_longlong(out.numel()))
+        if n < 0:
+            raise ValueError(f"page list export failed ({-n})")
+        return out.view(-1)[:total]
 
     def fill_block_table(self, seqs: list, table: torch.Tensor) -> None:
         """table: int32 CPU tensor [>= len(seqs), max_blocks], contiguous."""

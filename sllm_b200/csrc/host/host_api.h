@@ -34,6 +34,7 @@ SLLM_HOST_EXPORT long long sllm_kv_seq_length(int h, int seq);
 SLLM_HOST_EXPORT int sllm_kv_seq_pages(int h, int seq, int* out, int cap);
 SLLM_HOST_EXPORT int sllm_kv_seq_fork(int h, int seq, long long prefix_len, int* copy_pair);
 SLLM_HOST_EXPORT int sllm_kv_seq_make_tail_private(int h, int seq, int* copy_pair);
+SLLM_HOST_EXPORT long long sllm_kv_list_pages(int h, const int* seqs, const int* counts, int n, int* out, long long cap);
 SLLM_HOST_EXPORT int sllm_kv_fill_block_table(int h, const int* seqs, int n, int* table, int max_blocks);
 
 /* grammar.cpp */

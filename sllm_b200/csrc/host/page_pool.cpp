@@ -271,6 +271,27 @@ SLLM_HOST_EXPORT int sllm_kv_seq_make_tail_private(int h, int seq, int* copy_pai
   return 1;
 }
 
+// The first counts[i] pages of every sequence, one sequence after another.  Returns their number; nothing is written when they do not
+// fit in `cap` or a sequence has fewer.
+SLLM_HOST_EXPORT long long sllm_kv_list_pages(int h, const int* seqs, const int* counts, int n, int* out, long long cap) {
+  Pool* p = find_pool(h);
+  if (!p) return -SLLM_HOST_NOT_FOUND;
+  std::lock_guard<std::mutex> g(p->mu);
+  long long total = 0;
+  for (int i = 0; i < n; ++i) {
+    auto it = p->seqs.find(seqs[i]);
+    if (it == p->seqs.end()) return -SLLM_HOST_NOT_FOUND;
+    if (counts[i] < 0 || counts[i] > static_cast<int>(it->second.pages.size())) return -SLLM_HOST_INVALID;
+    total += counts[i];
+  }
+  if (total > cap) return -SLLM_HOST_LIMIT;
+  for (int i = 0; i < n; ++i) {
+    const std::vector<int>& pg = p->seqs.find(seqs[i])->second.pages;
+    out = std::copy(pg.begin(), pg.begin() + counts[i], out);
+  }
+  return total;
+}
+
 // Rows of the block table for `n` sequences; unused entries are set to 0 (a valid page index, never
 // read because kv_lens bounds every access).
 SLLM_HOST_EXPORT int sllm_kv_fill_block_table(int h, const int* seqs, int n, int* table, int max_blocks) {

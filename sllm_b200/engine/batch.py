@@ -8,8 +8,10 @@ which is why its batch planner was never connected (docs/plans/main-plan.md:894-
 from __future__ import annotations
 
 from dataclasses import dataclass, field
-from typing import Optional
+from itertools import chain
+from typing import Optional, Union
 
+import numpy as np
 import torch
 
 
@@ -37,15 +39,55 @@ class ForwardBatch:
     row_off_host: Optional[list] = None
     starts_host: Optional[list] = None
     plans: dict = field(default_factory=dict)  # device tables that ops derive from the structure, shared by the layers
+    staged_bytes: int = 0                      # copied to the device for this batch (eager batches)
 
     @property
     def num_tokens(self) -> int:
         return self.tokens.numel()
 
 
-def make_prefill_batch(prompts: list, block_table: torch.Tensor, device, start_positions: Optional[list] = None,
+@dataclass
+class PageLists:
+    """Pages of a batch's sequences up to their new lengths, one sequence after another (int32 CPU tensor): what the GPU makes a
+    block table of ``max_blocks`` columns from."""
+    pages: torch.Tensor
+    max_blocks: int
+    page_size: int
+
+
+def _planned_batch(prompts: list, table: Union[torch.Tensor, PageLists, None], device, starts: list, last_only: bool) -> ForwardBatch:
+    """`make_prefill_batch` on a GPU: one copy of tokens, lengths and pages, and one launch for everything that follows from them
+    (a prompt of 8192 tokens: positions and indexes as Python lists took several times its token list)."""
+    from .. import ops
+    lens = [len(p) for p in prompts]
+    t, s = sum(lens), len(lens)
+    paged = isinstance(table, PageLists)
+    pages = table.pages.numpy() if paged else np.empty(0, np.int32)
+    host = np.empty(t + 2 * s + pages.size, dtype=np.int32)
+    host[:t] = np.fromiter(chain.from_iterable(prompts), dtype=np.int32, count=t)
+    host[t:t + s], host[t + s:t + 2 * s], host[t + 2 * s:] = lens, starts, pages
+    tokens, new, begun, listed = torch.from_numpy(host).to(device).split_with_sizes((t, s, s, pages.size))
+    plan = ops.batch_plan(new, begun, listed, t, table.max_blocks if paged else 0, table.page_size if paged else 16)
+    cu = [0]
+    for n in lens:
+        cu.append(cu[-1] + n)
+    rows = None
+    if last_only:       # (an empty prompt's place is the row ahead of it)
+        rows = plan.last_rows if all(lens) else torch.tensor([c - 1 for c in cu[1:]], dtype=torch.int64, device=device)
+    fresh = not any(starts)
+    return ForwardBatch(tokens=tokens, positions=plan.positions, seq_index=plan.seq_index, kv_lens=plan.kv_lens,
+                        block_table=plan.block_table if paged else table, logit_rows=rows,
+                        max_kv=max((a + n for a, n in zip(starts, lens) if n), default=0), cu_seqlens=plan.row_off if fresh else None,
+                        max_seqlen=max(lens, default=0), cu_seqlens_host=cu if fresh else None, row_off=plan.row_off, row_off_host=cu,
+                        starts_host=list(starts), staged_bytes=host.nbytes)
+
+
+def make_prefill_batch(prompts: list, block_table: Union[torch.Tensor, PageLists, None], device, start_positions: Optional[list] = None,
                        last_only: bool = True) -> ForwardBatch:
-    """prompts: list of token-id lists, one per row of block_table."""
+    """prompts: list of token-id lists, one per row of block_table (on a GPU also `PageLists` in its place)."""
+    from ..ops.plan import MAX_REQUESTS
+    if torch.device(device).type == "cuda" and len(prompts) <= MAX_REQUESTS:
+        return _planned_batch(prompts, block_table, device, list(start_positions) if start_positions is not None else [0] * len(prompts), last_only)
     toks, pos, sidx = [], [], []
     cu = [0]
     rows = []

@@ -157,6 +157,12 @@ class LeaderEngine:
         self._ch.send(("embed", list(ids)))
         return self._e.embed_hidden(ids)
 
+    def score(self, prompts, top: int = 0, max_rows: int = Engine.SCORE_ROWS):
+        prompts = [list(p) for p in prompts]
+        self._e.check_score(prompts, top, max_rows)
+        self._ch.send(("score", prompts, top, max_rows))
+        return self._e.score(prompts, top, max_rows)
+
     def generate(self, prompts, max_new_tokens, eos=None, on_token=None):
         return Engine.generate(self, prompts, max_new_tokens, eos, on_token)
 
@@ -205,6 +211,8 @@ def _replay(engine: Engine, seqs: dict, cmd) -> None:
         engine.free_kv(cmd[1])
     elif op == "embed":
         engine.embed_hidden(cmd[1])
+    elif op == "score":
+        engine.score(cmd[1], cmd[2], cmd[3])
     elif op == "prefill_mm":
         batch = []
         for h, new_tokens in cmd[1]:

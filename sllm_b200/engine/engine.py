@@ -22,7 +22,7 @@ import torch
 from .. import ops
 from ..cache.paged import OutOfPages, PagedKVCache
 from ..models.config import ModelConfig
-from .batch import ForwardBatch, make_prefill_batch
+from .batch import ForwardBatch, PageLists, make_prefill_batch
 
 
 @dataclass
@@ -56,6 +56,9 @@ _PARKED: list = []
 
 class Engine:
     GRAPH_BATCHES = (1, 2, 4, 8, 16, 32, 64, 128)
+    # Entries from which a decode step sends its pages and has the GPU make the table of them (64 sequences of 1500 tokens, us a step with a
+    # new table: 131072 entries 271 from the host, 315 this way; 524288 entries 359 and 316)
+    WIDE_TABLE = 1 << 18
 
     def __init__(self, cfg: ModelConfig, model, cache: PagedKVCache, device, max_batch: int = 64,
                  use_cuda_graphs: bool = True, tp=None):
@@ -83,6 +86,7 @@ class Engine:
         self.d_seq_index = torch.arange(max_batch, dtype=torch.int32, device=self.device)
         self.d_table = torch.zeros((max_batch, self.max_blocks), dtype=torch.int32, device=self.device)
         self.d_out = torch.zeros(max_batch, dtype=torch.int32, device=self.device)
+        self.d_one = torch.ones(max_batch, dtype=torch.int32, device=self.device)
         self.h_slots = torch.zeros(max_batch, dtype=torch.int32, pin_memory=pin)
         self.d_slots = torch.zeros(max_batch, dtype=torch.int32, device=self.device)
         self.d_row_off = torch.arange(max_batch + 1, dtype=torch.int32, device=self.device)
@@ -214,9 +218,7 @@ class Engine:
         seq = self.new_sequence(ids)
         try:
             self.cache.pool.reserve(seq.seq_id, len(ids))
-            table = torch.zeros((1, self.max_blocks), dtype=torch.int32)
-            self.cache.pool.fill_block_table([seq.seq_id], table)
-            b = make_prefill_batch([list(ids)], table.to(self.device), self.device, last_only=False)
+            b = make_prefill_batch([list(ids)], self._table([seq], [len(ids)]), self.device, last_only=False)
             if self.has_state:
                 b.slots = self._slots([seq])
             h = self.model.hidden(b, self.cache)
@@ -225,6 +227,89 @@ class Engine:
             return ops.rmsnorm(h, self.model.w.final_norm, self.cfg.rms_eps, self.cfg.norm_offset_one)
         finally:
             self.free_sequence(seq)
+
+    SCORE_ROWS = 8192        # tokens of a forward pass of `score`
+
+    def score(self, prompts: list, top: int = 0, max_rows: int = SCORE_ROWS) -> list:
+        """What the model makes of given texts: per token list a `TokenLogprobs` on the CPU whose row i belongs to token i + 1 - its
+        log-probability after the tokens ahead of it, the entropy of that distribution and (with ``top``) its likeliest tokens.
+        Texts run together up to ``max_rows`` tokens, a longer one in portions, on scratch pages that are released again.  Without
+        ``top`` a dense output matrix on one GPU yields them without logits in memory, from unrounded sums; other heads go through
+        logits as `forward` gives them."""
+        self._guard()
+        prompts = [list(p) for p in prompts]
+        self.check_score(prompts, top, max_rows)
+        out, i = [], 0
+        while i < len(prompts):
+            j, rows = i + 1, len(prompts[i])
+            while j < len(prompts) and j - i < self.max_batch and rows + len(prompts[j]) <= max_rows:
+                rows += len(prompts[j])
+                j += 1
+            out += self._score_together(prompts[i:j], top, max_rows)
+            i = j
+        return out
+
+    def check_score(self, prompts: list, top: int, max_rows: int) -> None:
+        """Raises for arguments that `score` refuses."""
+        if any(not 1 <= len(p) <= self.cfg.max_context or min(p) < 0 or max(p) >= self.cfg.vocab for p in prompts):
+            raise ValueError("a scored text has between one token and the context's length, all inside the vocabulary")
+        if not 0 <= top <= ops.logprobs.MAX_TOP or max_rows < 1:
+            raise ValueError(f"top lies between 0 and {ops.logprobs.MAX_TOP}, max_rows at 1 or more")
+
+    def _score_together(self, prompts: list, top: int, max_rows: int) -> list:
+        pool, seqs, found = self.cache.pool, [], [[] for _ in prompts]
+        try:
+            for p in prompts:
+                seqs.append(self.new_sequence(p))
+            for start in range(0, max(map(len, prompts)), max_rows):       # (several portions: of a single text)
+                parts = [p[start:start + max_rows] for p in prompts]
+                ends = [start + len(part) for part in parts]
+                for s, n in zip(seqs, ends):
+                    pool.reserve(s.seq_id, n)
+                b = make_prefill_batch(parts, self._table(seqs, ends), self.device, [start] * len(seqs), last_only=False)
+                if self.has_state:
+                    b.slots = self._slots(seqs)
+                self.h2d_bytes += b.staged_bytes or b.num_tokens * 12
+                h = self.model.hidden(b, self.cache)
+                counts = [min(n, len(p) - 1) - start for n, p in zip(ends, prompts)]      # rows with a token behind them
+                at = [r0 + k for r0, n in zip(b.row_off_host, counts) for k in range(n)]
+                if at:
+                    tokens = [p[start + k + 1] for p, n in zip(prompts, counts) for k in range(n)]
+                    idx = torch.tensor([at, tokens], dtype=torch.int64).to(self.device)
+                    got = [None if f is None else f.cpu() for f in self._row_logprobs(b, h, idx[0], idx[1], top)]
+                    self.d2h_bytes += sum(f.numel() * 4 for f in got if f is not None)
+                    r0 = 0
+                    for f, n in zip(found, counts):
+                        f.append([None if g is None else g[r0:r0 + n] for g in got])
+                        r0 += n
+                for s, n in zip(seqs, ends):
+                    pool.commit(s.seq_id, n)
+                    s.num_computed = n
+            self._check_status(every=1)
+        finally:
+            for s in seqs:
+                self.free_sequence(s)
+        none = ops.token_logprobs(torch.empty((0, 1)), torch.empty(0, dtype=torch.int64), top) if any(not f for f in found) else None
+        return [ops.TokenLogprobs(*(None if g[0] is None else torch.cat(g) for g in zip(*f))) if f else none for f in found]
+
+    def _row_logprobs(self, b: ForwardBatch, h: torch.Tensor, rows: torch.Tensor, tokens: torch.Tensor, top: int):
+        """`ops.TokenLogprobs` of ``tokens`` after the rows ``rows`` of the residual ``h``."""
+        m, cfg = self.model, self.cfg
+        if not top and m.tp.size == 1 and m.w.lm_head.kind == "dense":
+            if hasattr(m, "final_hidden"):
+                x = m.final_hidden(h, rows)
+            else:
+                x = ops.rmsnorm(h.index_select(0, rows), m.w.final_norm, cfg.rms_eps, cfg.norm_offset_one)
+            capped = cfg.family in ("llama", "gemma4", "sepedra")          # families whose logits pass the soft cap
+            return ops.linear_logprobs(x, m.w.lm_head, tokens, softcap=cfg.logit_softcap if capped else 0.0)
+        parts, step = [], max(1, ops.logprobs.CHUNK_LOGITS // cfg.vocab)
+        for lo in range(0, rows.numel(), step):
+            b.logit_rows = rows[lo:lo + step]
+            z = m.logits(h, b)
+            if z.shape[1] != cfg.vocab:
+                z = m.tp.gather_logits(z)
+            parts.append(ops.token_logprobs(z, tokens[lo:lo + step], top))
+        return ops.TokenLogprobs(*(None if f[0] is None else torch.cat(f) for f in zip(*parts)))
 
     def shutdown_report(self) -> dict:
         """What a supervisor logs when the engine goes away: memory by category, launch and copy counters, fallbacks
@@ -236,6 +321,18 @@ class Engine:
                 "kv_pool": self.cache.pool.stats() if hasattr(self.cache, "pool") else None}
 
     # ------------------------------------------------------------------ sequences
+    def _table(self, seqs: list, lengths: list):
+        """Where the first lengths[i] tokens of each sequence lie, for `make_prefill_batch`."""
+        pool, ids = self.cache.pool, [s.seq_id for s in seqs]
+        if self.is_cuda:
+            if any(n > self.max_blocks * self.cfg.page_size for n in lengths):
+                raise ValueError("a sequence is longer than the block table")
+            return PageLists(pool.list_pages(ids, lengths), self.max_blocks, self.cfg.page_size)
+        table = torch.zeros((len(seqs), self.max_blocks), dtype=torch.int32)
+        pool.fill_block_table(ids, table)
+        self.h2d_bytes += table.numel() * 4
+        return table
+
     def _slots(self, seqs: list) -> torch.Tensor:
         return torch.tensor([self.cache.slot_of[s.seq_id] for s in seqs], dtype=torch.int32, device=self.device)
 
@@ -357,10 +454,6 @@ class Engine:
         pool = self.cache.pool
         for s in seqs:
             pool.reserve(s.seq_id, len(s.tokens))
-        table = torch.zeros((len(seqs), self.max_blocks), dtype=torch.int32)
-        pool.fill_block_table([s.seq_id for s in seqs], table)
-        d_table = table.to(self.device, non_blocking=True) if self.is_cuda else table
-        self.h2d_bytes += table.numel() * 4
         starts = [s.num_computed for s in seqs]
         budget = chunk_tokens if chunk_tokens > 0 else max(len(s.tokens) for s in seqs)
         out = None
@@ -374,8 +467,8 @@ class Engine:
                     rows.append(i)
             if not parts:
                 break
-            sub_table = d_table if len(rows) == len(seqs) else d_table[torch.tensor(rows, device=d_table.device)]
-            b = make_prefill_batch(parts, sub_table, self.device, part_starts)
+            b = make_prefill_batch(parts, self._table([seqs[i] for i in rows], [a + len(p) for a, p in zip(part_starts, parts)]), self.device,
+                                   part_starts)
             if embeds is not None:
                 b.embeds = embeds
             if rope_pos3 is not None:
@@ -389,7 +482,7 @@ class Engine:
                 b.rope_pos3 = self._rope3_rows([seqs[i] for i in rows], [len(p) for p in parts], b.positions)
             if self.has_state:
                 b.slots = self._slots([seqs[i] for i in rows])
-            self.h2d_bytes += b.num_tokens * 12
+            self.h2d_bytes += b.staged_bytes or b.num_tokens * 12
             res = self.model.greedy(b, self.cache) if sample else self.model.forward(b, self.cache)
             if self.keep_hidden:
                 self._log_hidden([seqs[i] for i in rows], part_starts, [len(p) for p in parts], self.model.last_hidden)
@@ -418,9 +511,6 @@ class Engine:
         pool = self.cache.pool
         for s in seqs:
             pool.reserve(s.seq_id, len(s.tokens))
-        table = torch.zeros((len(seqs), self.max_blocks), dtype=torch.int32)
-        pool.fill_block_table([s.seq_id for s in seqs], table)
-        d_table = table.to(self.device, non_blocking=True) if self.is_cuda else table
         parts = [s.tokens[s.num_computed:] for s in seqs]
         if any(not p for p in parts):
             raise ValueError("extend needs at least one uncomputed token per sequence")
@@ -428,14 +518,14 @@ class Engine:
         if (sample and self.use_graphs and not self.has_state and embeds is None and r <= self.MAX_EXTEND_ROWS
                 and not any(s.rope_delta for s in seqs)
                 and len(seqs) <= self.max_batch and all(len(p) == r for p in parts)):
-            return self._extend_graphed(seqs, parts, r, table)
-        b = make_prefill_batch(parts, d_table, self.device, [s.num_computed for s in seqs], last_only=False)
+            return self._extend_graphed(seqs, parts, r)
+        b = make_prefill_batch(parts, self._table(seqs, [len(s.tokens) for s in seqs]), self.device, [s.num_computed for s in seqs], last_only=False)
         b.embeds = embeds
         if self.cfg.mrope_sections and any(s.rope_delta for s in seqs):
             b.rope_pos3 = self._rope3_rows(seqs, [len(p) for p in parts], b.positions)
         if self.has_state:
             b.slots = self._slots(seqs)
-        self.h2d_bytes += table.numel() * 4 + b.num_tokens * 12
+        self.h2d_bytes += b.staged_bytes or b.num_tokens * 12
         res = self.model.greedy(b, self.cache) if sample else self.model.forward(b, self.cache)
         if self.keep_hidden:
             self._log_hidden(seqs, [s.num_computed for s in seqs], [len(p) for p in parts], self.model.last_hidden)
@@ -471,9 +561,7 @@ class Engine:
         pool = self.cache.pool
         for s in seqs:
             pool.reserve(s.seq_id, len(s.tokens))
-        table = torch.zeros((len(seqs), self.max_blocks), dtype=torch.int32)
-        pool.fill_block_table([s.seq_id for s in seqs], table)
-        b = make_prefill_batch([s.tokens[s.num_computed:] for s in seqs], table.to(self.device), self.device,
+        b = make_prefill_batch([s.tokens[s.num_computed:] for s in seqs], self._table(seqs, [len(s.tokens) for s in seqs]), self.device,
                                [s.num_computed for s in seqs])
         rows = [r0 + p for r0, w in zip(b.row_off_host, wanted) for p in w]
         b.logit_rows = torch.tensor(rows, dtype=torch.int64, device=self.device)
@@ -481,7 +569,7 @@ class Engine:
             b.rope_pos3 = self._rope3_rows(seqs, counts, b.positions)
         if self.has_state:
             b.slots = self._slots(seqs)
-        self.h2d_bytes += table.numel() * 4 + b.num_tokens * 12
+        self.h2d_bytes += b.staged_bytes or b.num_tokens * 12
         if rows:
             out = self.model.forward(b, self.cache)
         else:
@@ -498,10 +586,12 @@ class Engine:
 
     MAX_EXTEND_ROWS = 9      # a verify block: the last committed token plus up to 8 drafts
 
-    def _extend_graphed(self, seqs: list, parts: list, r: int, table: torch.Tensor):
+    def _extend_graphed(self, seqs: list, parts: list, r: int):
         """`extend` for equally long blocks (speculative verify) replayed from a CUDA graph per (sequences, rows)."""
         n = len(seqs)
         t = n * r
+        if self._staged is not None:
+            self._staged.synchronize()       # a decode step that nobody read back may still be copying out of h_table
         if getattr(self, "_ext", None) is None:
             cap = self.max_batch * self.MAX_EXTEND_ROWS
             pin = self.is_cuda
@@ -515,7 +605,7 @@ class Engine:
         flat_pos = [s.num_computed + i for s in seqs for i in range(r)]
         e["h_tok"][:t] = torch.tensor(flat_tok, dtype=torch.int32)
         e["h_pos"][:t] = torch.tensor(flat_pos, dtype=torch.int32)
-        self.h_table[:n].copy_(table)
+        self.cache.pool.fill_block_table([s.seq_id for s in seqs], self.h_table)
         self.d_table[:n].copy_(self.h_table[:n], non_blocking=True)
         self._table_key = None
         e["d_tok"][:t].copy_(e["h_tok"][:t], non_blocking=True)
@@ -658,7 +748,15 @@ class Engine:
             self.np_positions[n:np_] = self.np_positions[0]
         # The block table changes only when a sequence crosses a page boundary or the batch changes.
         key = (tuple(s.seq_id for s in seqs), tuple((len(s.tokens) + ps - 1) // ps for s in seqs))
-        if key != self._table_key:
+        self.d_positions[:np_].copy_(self.h_positions[:np_], non_blocking=True)
+        if key != self._table_key and self.is_cuda and np_ * self.max_blocks >= self.WIDE_TABLE:
+            lens = self.np_positions[:np_] + 1
+            pages = pool.list_pages([s.seq_id for s in seqs] + [seqs[0].seq_id] * (np_ - n), lens.tolist(), out=self.h_table)
+            d_pages = torch.empty(pages.numel(), dtype=torch.int32, device=self.device).copy_(pages, non_blocking=True)
+            ops.batch_plan(self.d_one[:np_], self.d_positions[:np_], d_pages, np_, self.max_blocks, ps, table=self.d_table[:np_])
+            self.h2d_bytes += pages.numel() * 4
+            self._table_key = key
+        elif key != self._table_key:
             pool.fill_block_table([s.seq_id for s in seqs], self.h_table)
             if np_ > n:
                 self.h_table[n:np_] = self.h_table[0]
@@ -672,7 +770,6 @@ class Engine:
             self.h_slots[:n] = torch.tensor([self.cache.slot_of[s.seq_id] for s in seqs], dtype=torch.int32)
             self.d_slots[:n].copy_(self.h_slots[:n], non_blocking=True)
         self.d_tokens[:np_].copy_(self.h_tokens[:np_], non_blocking=True)
-        self.d_positions[:np_].copy_(self.h_positions[:np_], non_blocking=True)
         torch.add(self.d_positions[:np_], 1, out=self.d_kv_lens[:np_])
         self.h2d_bytes += np_ * 8
         self._rope3_on = bool(self.cfg.mrope_sections) and any(s.rope_delta for s in seqs)

@@ -12,14 +12,15 @@ import torch
 from .config import ModelConfig
 
 # CUDA translation units of a family, for callers that build no more than they run (None: the whole library)
+_ENGINE = ("batch_plan", "logprobs", "head_logprobs")       # of the engine's batches and of `score`
 KERNEL_UNITS = {
-    "zokuvik": ("elementwise", "gemm_tcgen05", "gemm_prompt", "gemm_simt", "group_norm", "latent_attention", "latent_decode", "latent_prefill",
+    "zokuvik": _ENGINE + ("elementwise", "gemm_tcgen05", "gemm_prompt", "gemm_simt", "group_norm", "latent_attention", "latent_decode", "latent_prefill",
                 "delta_rule", "state_scan"),
-    "sepedra": ("elementwise", "gemm_tcgen05", "gemm_prompt", "gemm_simt", "group_norm", "attention", "kv_attention", "short_conv", "latent_prefill", "rglru", "moe",
+    "sepedra": _ENGINE + ("elementwise", "gemm_tcgen05", "gemm_prompt", "gemm_simt", "group_norm", "attention", "kv_attention", "short_conv", "latent_prefill", "rglru", "moe",
                 "moe_dense"),
-    "kegorax": ("elementwise", "gemm_tcgen05", "gemm_prompt", "gemm_simt", "group_norm", "attention", "kv_attention", "short_conv", "latent_prefill",
+    "kegorax": _ENGINE + ("elementwise", "gemm_tcgen05", "gemm_prompt", "gemm_simt", "group_norm", "attention", "kv_attention", "short_conv", "latent_prefill",
                 "linear_state", "state_scan", "moe", "moe_dense"),
-    "fekolorn": ("elementwise", "gemm_tcgen05", "gemm_prompt", "gemm_simt", "hyper_streams", "poly_norm", "attention", "kv_attention", "short_conv",
+    "fekolorn": _ENGINE + ("elementwise", "gemm_tcgen05", "gemm_prompt", "gemm_simt", "hyper_streams", "poly_norm", "attention", "kv_attention", "short_conv",
                  "latent_prefill", "linear_state", "state_scan"),
 }
 

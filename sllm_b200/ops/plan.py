@@ -76,9 +76,11 @@ def batch_plan(new_lens: torch.Tensor, starts: torch.Tensor, pages: torch.Tensor
                     torch.empty((s, max_blocks), dtype=torch.int32) if table is None else table)
     # (one allocation: a tensor of its own for each part costs more than the kernel)
     cells = 0 if table is not None else s * max_blocks
-    n32 = cells + s + 1 + 3 * rows
-    rest, slots, last_rows = torch.empty(n32 // 2 + 1 + rows + s, dtype=torch.int64, device=dev).split_with_sizes((n32 // 2 + 1, rows, s))
-    own, row_off, positions, seq_index, kv_lens, _ = rest.view(torch.int32).split_with_sizes((cells, s + 1, rows, rows, rows, 2 - n32 % 2))
+    ca, sa, ra, la = -cells % 4, -(s + 1) % 4, -rows % 4, -rows % 2      # (every part starts at 16 bytes)
+    half = (cells + ca + s + 1 + sa + 3 * (rows + ra)) // 2
+    rest, slots, _, last_rows = torch.empty(half + rows + la + s, dtype=torch.int64, device=dev).split_with_sizes((half, rows, la, s))
+    own, _, row_off, _, positions, _, seq_index, _, kv_lens, _ = rest.view(torch.int32).split_with_sizes(
+        (cells, ca, s + 1, sa, rows, ra, rows, ra, rows, ra))
     if table is None:
         table = own.view(s, max_blocks)
     rc = _launch(dev, _k().sllm_batch_plan, new_lens.data_ptr(), starts.data_ptr(), pages.data_ptr(), pages.numel(), s, rows, max_blocks,
