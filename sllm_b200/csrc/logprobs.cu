@@ -142,12 +142,6 @@ __device__ __forceinline__ float lp_exp2(float x) {            // 0 below the sm
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-__device__ __forceinline__ uint64_t lp_add2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-
 // A load that stays where it is written, so that several are under way at a time; the row passes L1 by.
 __device__ __forceinline__ uint4 lp_stream(const uint4* p) {
   uint4 r;
@@ -278,7 +272,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(con
       const uint64_t t2 = fma_f32x2(pack_f32x2(x.x, x.y), scale, ref);
       const float2 t = unpack_f32x2(t2);
       const uint64_t e2 = pack_f32x2(lp_exp2(t.x), lp_exp2(t.y));
-      s2 = lp_add2(s2, e2);
+      s2 = add_f32x2(s2, e2);
       w2 = fma_f32x2(e2, t2, w2);
     }
   };
