@@ -154,7 +154,8 @@ constexpr float kLpSlack = 4.f;            // a thread's sums are taken anew whe
 
 constexpr int kLpMaxCluster = 8;
 constexpr int kLpSmallUnits = 1024;
-constexpr int kLpFill = 1184;
+constexpr int kLpFill = 640;                // CTAs of 256 threads from which a row has one of its own (the card holds 592)
+constexpr int kLpLongRows = 2368;
 constexpr int kLpMaxVocab = 1 << 30;       // ids and units stay below 2^31
 
 // Sums of one part of a row with respect to m.
@@ -181,15 +182,17 @@ struct LpStats {
   }
 };
 
+constexpr int kLpParts = 4;                // of a range, with a maximum per thread each
 constexpr int kLpPool = 256;               // candidates that are ranked against one another
 
-template <int kThreads>
+template <int kThreads, int kParts>
 struct __align__(16) LpShared {
   static constexpr int kWarps = kThreads / 32;
   LpStats stat[kWarps];
   float high[32];                          // the largest of the threads' maxima of each warp
   int wins, count;
-  unsigned char win[kThreads];             // threads with logits at or above the bound
+  float best[kParts][kThreads];          // the largest logit of a thread's units by part of the range
+  unsigned short win[kParts * kThreads]; // parts with logits at or above the bound: part kThreads + thread
   LpKey pool[kLpPool];
   LpKey merged[kWarps][32];
   LpKey list[32];                          // the CTA's alternatives
@@ -201,13 +204,15 @@ struct __align__(16) LpShared {
 // A cluster of CTAs per row (one where there are many rows), each with a range of the row's 16-byte units; unit v of a range goes to
 // thread v mod kThreads.  One pass takes S and W per thread with respect to a reference that follows the maximum loosely, so that the
 // usual unit has no branch, and the thread's largest logit.
-// Alternatives: the top-th largest of the threads' maxima bounds the wanted ones from below, and hardly more threads have logits at or
-// above it than there are alternatives; those threads' units are read again (out of L2) and what passes the bound is ranked by
+// Alternatives: the top-th largest of the threads' maxima bounds the wanted ones from below, and hardly more parts of threads' units have
+// logits at or above it than there are alternatives; those units are read again (out of L2) and what passes the bound is ranked by
 // counting.  Where more than kLpPool logits pass it (runs of equal or ordered ones), sorted lists are merged 32 at a time instead.
-template <typename T, int kThreads, bool kTop>
+// kLong, for many long rows: rounds of loads without a bound, and the maxima of kLpParts parts of a thread's units, so that less is read
+// again (4096 x 128256 bf16, us: without alternatives 190 -> 184, 5 of them 214 -> 207, 32 of them 316 -> 257; with 700 rows 5 take 43.5 -> 45.3).
+template <typename T, int kThreads, bool kTop, bool kLong>
 __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(const LogprobParams p, int cluster) {
-  constexpr int kN = LpVec<T>::kN, kWarps = kThreads / 32, kAhead = 4;
-  __shared__ LpShared<kThreads> sh;
+  constexpr int kN = LpVec<T>::kN, kWarps = kThreads / 32, kAhead = 4, kParts = kLong ? kLpParts : 1;
+  __shared__ LpShared<kThreads, kParts> sh;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
   const int rank = cluster > 1 ? static_cast<int>(blockIdx.x % cluster) : 0;
   const long long row = blockIdx.x / cluster;
@@ -276,22 +281,62 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(con
       w2 = fma_f32x2(e2, t2, w2);
     }
   };
+  const int each = (hi - lo + kThreads - 1) / kThreads;        // units per thread; per part, in whole rounds of loads
+  const int part_units = kParts > 1 ? max((each + kParts * kAhead - 1) / (kParts * kAhead), 1) * kAhead : max(each, 1);
   if (lo + tid < min(hi, whole_lo)) add(load_unit(lo + tid));
   // (whole_lo is at most 1: only thread 0 of the first range has such a unit, and goes on behind it)
   const int end = min(hi, whole_hi);
-  for (int v = lo + tid + (lo + tid < whole_lo ? kThreads : 0); v < end; v += kAhead * kThreads) {
-    LpVec<T> u[kAhead];
+  int v = lo + tid + (lo + tid < whole_lo ? kThreads : 0);
+  if constexpr (!kLong) {
+    for (; v < end; v += kAhead * kThreads) {
+      LpVec<T> u[kAhead];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      u[i].raw = make_uint4(lp_shut<T>(), lp_shut<T>(), lp_shut<T>(), lp_shut<T>());
-      if (v + i * kThreads < end) u[i].raw = lp_stream(units + v + i * kThreads);
+      for (int i = 0; i < kAhead; ++i) {
+        u[i].raw = make_uint4(lp_shut<T>(), lp_shut<T>(), lp_shut<T>(), lp_shut<T>());
+        if (v + i * kThreads < end) u[i].raw = lp_stream(units + v + i * kThreads);
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) add(u[i]);
     }
+  } else {
+#pragma unroll 1
+    for (int part = 0; part < kParts; ++part) {
+      const int stop = min(end, lo + (part + 1) * part_units * kThreads);
+      for (; v + (kAhead - 1) * kThreads < stop; v += kAhead * kThreads) {
+        LpVec<T> u[kAhead];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) add(u[i]);
+        for (int i = 0; i < kAhead; ++i) u[i].raw = lp_stream(units + v + i * kThreads);
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) add(u[i]);
+      }
+      if (v < stop) {
+        LpVec<T> u[kAhead - 1];
+#pragma unroll
+        for (int i = 0; i < kAhead - 1; ++i) {
+          u[i].raw = make_uint4(lp_shut<T>(), lp_shut<T>(), lp_shut<T>(), lp_shut<T>());
+          if (v + i * kThreads < stop) u[i].raw = lp_stream(units + v + i * kThreads);
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead - 1; ++i) add(u[i]);
+      }
+      v = lo + tid + (part + 1) * part_units * kThreads;       // (a thread that began one unit later goes on with the others)
+      sh.best[part][tid] = best;
+      if (kTop) best = kNone;
+    }
   }
   {
     const int v = n_units - 1;                                 // the last unit, where it is not whole and was not the first as well
-    if (v >= whole_hi && v >= whole_lo && v >= lo && v < hi && (v - lo) % kThreads == tid) add(load_unit(v));
+    if (v >= whole_hi && v >= whole_lo && v >= lo && v < hi && (v - lo) % kThreads == tid) {
+      add(load_unit(v));
+      if constexpr (kTop && kLong) {
+        float& its = sh.best[(v - lo) / kThreads / part_units][tid];
+        its = fmaxf(its, best);
+      }
+    }
+  }
+  if constexpr (kTop && kLong) {
+#pragma unroll
+    for (int part = 0; part < kParts; ++part) best = fmaxf(best, sh.best[part][tid]);
   }
 
   float tok_x = logit(tok);
@@ -372,11 +417,19 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(con
     if (lane < kHigh) sh.high[warp * kHigh + lane] = v;
     __syncthreads();
     const float bound = __shfl_sync(0xffffffffu, lp_sort(sh.high[lane]), p.top - 1);      // -inf: every token counts
-    if (best >= bound && best > -INFINITY) sh.win[atomicAdd(&sh.wins, 1)] = static_cast<unsigned char>(tid);
+#pragma unroll
+    for (int part = 0; part < kParts; ++part) {
+      const float x = kLong ? sh.best[part][tid] : best;
+      if (x >= bound && x > -INFINITY) sh.win[atomicAdd(&sh.wins, 1)] = static_cast<unsigned short>(part * kThreads + tid);
+    }
     __syncthreads();
-    // the winners' units, dealt out over all threads
-    const int each = (hi - lo + kThreads - 1) / kThreads, todo = sh.wins * each;
-    auto unit_of = [&](int i) { return i < todo ? lo + sh.win[i / each] + i % each * kThreads : hi; };      // hi: none
+    // their units, dealt out over all threads
+    const int todo = sh.wins * part_units;
+    auto unit_of = [&](int i) {                                // beyond the range: none
+      if (i >= todo) return hi;
+      const int win = sh.win[i / part_units];
+      return lo + win % kThreads + (win / kThreads * part_units + i % part_units) * kThreads;
+    };
     for (int i0 = tid; i0 < todo; i0 += kAhead * kThreads) {
       LpVec<T> u[kAhead];
       int at[kAhead];
@@ -486,17 +539,21 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(con
   }
 }
 
-template <typename T, int kThreads>
+template <typename T, int kThreads, bool kLong = false>
 static cudaError_t logprobs_go(const LogprobParams& p, int cluster, cudaStream_t st) {
   const dim3 grid(static_cast<unsigned>(p.rows) * cluster), block(kThreads);
-  return p.top ? launch_kernel_cluster(logprobs_kernel<T, kThreads, true>, grid, block, 0, st, cluster, 1u, p, cluster)
-               : launch_kernel_cluster(logprobs_kernel<T, kThreads, false>, grid, block, 0, st, cluster, 1u, p, cluster);
+  return p.top ? launch_kernel_cluster(logprobs_kernel<T, kThreads, true, kLong>, grid, block, 0, st, cluster, 1u, p, cluster)
+               : launch_kernel_cluster(logprobs_kernel<T, kThreads, false, kLong>, grid, block, 0, st, cluster, 1u, p, cluster);
 }
 
+// us a launch that decide: many rows of up to kLpSmallUnits units go to CTAs of 64 threads (2655 x 6135 bf16: 9.5, with 256 threads 18.9), few
+// of them do not (138 x 2067 fp32 with 32 alternatives: 9.5 and 6.9).  Rows are shared by a cluster where they would not give every SM
+// four CTAs (100 x 128256 bf16 with 5 alternatives: 13.6 in clusters of four, 17.9 of eight; 300: 27.7 in clusters of two, 31.0 alone).
 template <typename T>
 static cudaError_t logprobs_go(const LogprobParams& p, cudaStream_t st) {
   const long long units = (static_cast<long long>(p.vocab) + LpVec<T>::kN - 1) / LpVec<T>::kN;
-  if (units <= kLpSmallUnits) return logprobs_go<T, 64>(p, 1, st);
+  if (units <= 256 || (units <= kLpSmallUnits && p.rows > kLpFill)) return logprobs_go<T, 64>(p, 1, st);
+  if (p.rows >= kLpLongRows && units >= 32 * 256) return logprobs_go<T, 256, true>(p, 1, st);
   int cluster = 1;
   while (cluster < kLpMaxCluster && static_cast<long long>(p.rows) * cluster * 2 <= kLpFill && units >= 2 * cluster * 256) cluster *= 2;
   return logprobs_go<T, 256>(p, cluster, st);

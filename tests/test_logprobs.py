@@ -179,7 +179,7 @@ def test_the_head_launcher_refuses():
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("r,v,gap,shift,top", [(1, 1, 0, 0, 3), (2, 5, 3, 1, 2), (3, 31, 0, 0, 32), (5, 257, 1, 1, 1), (4, 2048, 0, 0, 5),
                                                (7, 4099, 5, 3, 20), (1, 32000, 0, 0, 32), (300, 1000, 24, 8, 4), (700, 515, 0, 1, 0), (2, 131077, 11, 7, 20),
-                                               (160, 9001, 0, 0, 7)])
+                                               (160, 9001, 0, 0, 7), (650, 9001, 5, 3, 6), (1250, 8400, 0, 0, 0), (593, 12289, 7, 1, 32)])
 def test_kernel_matches_the_definition(dtype, r, v, gap, shift, top):
     z, ids = rows(r, v, dtype, r * v, gap, shift, device=DEV)
     check(z, ids, top, ops.token_logprobs(z, ids.int() if r % 2 else ids, top))
@@ -196,6 +196,51 @@ def test_kernel_at_the_edges(dtype, v, top):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,v", [(torch.bfloat16, 65543), (torch.bfloat16, 70001), (torch.float32, 32771)])
+@pytest.mark.parametrize("top", [0, 6, 32])
+def test_many_long_rows(dtype, v, top):
+    """Rows enough for the kernel that takes them in parts: a sample of them against the definition, all of them against the kernel for
+    fewer (the order of additions is the same, the alternatives are whole numbers and values of the logits)."""
+    r = 2400
+    store = torch.randn(r * v + 5, device=DEV, generator=torch.Generator(device=DEV).manual_seed(v)).mul_(2.5).to(dtype)
+    z = store[5:].view(r, v)
+    z[7] = special(v, dtype)[8].to(DEV)
+    z[8] = -INF
+    z[9, 100:] = -INF
+    z[10] = 1.0
+    z[11] = torch.arange(v, device=DEV) / 256
+    ids = torch.randint(0, v, (r,), device=DEV)
+    got = ops.token_logprobs(z, ids, top)
+    few = slice(5, 13)
+    check(z[few], ids[few], top, ops.TokenLogprobs(*(None if f is None else f[few] for f in got)))
+    for lo in range(0, r, 600):
+        part = slice(lo, lo + 600)
+        want = ops.token_logprobs(z[part], ids[part], top)
+        for a, b in zip(got, want):
+            assert a is None or torch.allclose(a[part].double(), b.double(), rtol=1e-5, atol=1e-4, equal_nan=True)
+        assert not top or torch.equal(got.top_ids[part], want.top_ids)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("top", [0, 6])
+def test_many_rows_at_the_edges(dtype, top):
+    """Rows of every kind one after another in the same CTAs."""
+    v = 9007
+    one = special(v, dtype)
+    z = one.repeat(60, 1).to(DEV)
+    ids = torch.randint(-1, v + 1, (13, 2), generator=torch.Generator().manual_seed(1)).to(DEV)
+    got = ops.token_logprobs(z, ids.repeat(60, 1), top)
+    for k in (0, 31, 59):
+        part = ops.TokenLogprobs(*(None if f is None else f[13 * k:13 * k + 13] for f in got))
+        check(one, ids, top, part)
+    # a row's sums go by its 16-byte units, so rows of one alignment (8 x 13 apart: 8 x 9007 elements are whole units) have the same bits
+    for k in (8, 56):
+        assert all(f is None or torch.equal(torch.nan_to_num(f[13 * k:13 * k + 13]), torch.nan_to_num(f[:13])) for f in got)
+    assert ops.device_status(z.device) == 0
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("order", ["rising", "falling", "equal", "runs", "few"])
 @pytest.mark.parametrize("v", [700, 40000])
 def test_alternatives_of_ordered_rows(order, v):
@@ -209,6 +254,8 @@ def test_alternatives_of_ordered_rows(order, v):
         got = ops.token_logprobs(x, ids, 32)
         _, _, tid, _ = oracle(x, ids, 32)
         assert torch.equal(got.top_ids.cpu().long(), tid)
+        got = ops.token_logprobs(x.repeat(300, 1), ids.repeat(300), 32)
+        assert torch.equal(got.top_ids.cpu().long(), tid.repeat(300, 1))
 
 
 @pytest.mark.gpu
