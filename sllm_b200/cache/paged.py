@@ -129,12 +129,14 @@ class PagePool:
         self._lib.sllm_kv_pool_inject_alloc_failure(self.h, after_calls)
 
     def list_pages(self, seqs: list, lengths: list, out=None):
-        """Pages that hold the first lengths[i] tokens of every sequence, one sequence after another: an int32 array, a part of
+        """Pages that hold the first lengths[i] tokens of every sequence, one sequence after another: int32, the head of
         ``out`` (a contiguous int32 CPU tensor) where one is given."""
         counts = [(n + self.page_size - 1) // self.page_size for n in lengths]
         total = sum(counts)
         if out is None:
             out = torch.empty(total, dtype=torch.int32)
+        elif out.dtype != torch.int32 or out.device.type != "cpu" or not out.is_contiguous():
+            raise ValueError("pages are listed into a contiguous int32 CPU tensor")
         arr = (C.c_int * len(seqs))(*seqs)
         n = self._lib.sllm_kv_list_pages(self.h, arr, (C.c_int * len(seqs))(*counts), len(seqs), C.c_void_p(out.data_ptr()),
                                          C.c_longlong(out.numel()))

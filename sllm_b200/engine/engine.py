@@ -289,8 +289,8 @@ class Engine:
         finally:
             for s in seqs:
                 self.free_sequence(s)
-        none = ops.token_logprobs(torch.empty((0, 1)), torch.empty(0, dtype=torch.int64), top) if any(not f for f in found) else None
-        return [ops.TokenLogprobs(*(None if g[0] is None else torch.cat(g) for g in zip(*f))) if f else none for f in found]
+        none = [torch.empty(0), torch.empty(0), torch.empty((0, top), dtype=torch.int32) if top else None, torch.empty((0, top)) if top else None]
+        return [ops.TokenLogprobs(*(None if g[0] is None else torch.cat(g) for g in zip(*f))) if f else ops.TokenLogprobs(*none) for f in found]
 
     def _row_logprobs(self, b: ForwardBatch, h: torch.Tensor, rows: torch.Tensor, tokens: torch.Tensor, top: int):
         """`ops.TokenLogprobs` of ``tokens`` after the rows ``rows`` of the residual ``h``."""
@@ -751,6 +751,8 @@ class Engine:
         self.d_positions[:np_].copy_(self.h_positions[:np_], non_blocking=True)
         if key != self._table_key and self.is_cuda and np_ * self.max_blocks >= self.WIDE_TABLE:
             lens = self.np_positions[:np_] + 1
+            if int(lens.max()) > self.max_blocks * ps:
+                raise ValueError("a sequence is longer than the block table")
             pages = pool.list_pages([s.seq_id for s in seqs] + [seqs[0].seq_id] * (np_ - n), lens.tolist(), out=self.h_table)
             d_pages = torch.empty(pages.numel(), dtype=torch.int32, device=self.device).copy_(pages, non_blocking=True)
             ops.batch_plan(self.d_one[:np_], self.d_positions[:np_], d_pages, np_, self.max_blocks, ps, table=self.d_table[:np_])

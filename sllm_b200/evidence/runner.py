@@ -215,10 +215,61 @@ def _moe_route(size):
     return (lambda: M.route(logits, k)[1]), want, 2 * t * e, 0, {"tokens": t, "experts": e, "top_k": k}, (1e-4, 1e-5)
 
 
+def _token_logprobs(size):
+    import torch
+    from .. import ops
+    rows, v, top = {"small": (8, 4096, 5), "decode": (64, 128256, 20), "large": (2048, 128256, 5)}[size]
+    z = torch.randn(rows, v, device="cuda").bfloat16()
+    ids = torch.randint(0, v, (rows,), device="cuda")
+
+    def run():
+        p = ops.token_logprobs(z, ids, top)
+        return torch.cat([p.logprob[:, None], p.entropy[:, None], p.top_logprobs], 1)
+
+    p = ops.token_logprobs(z.cpu(), ids.cpu(), top)
+    return (run, torch.cat([p.logprob[:, None], p.entropy[:, None], p.top_logprobs], 1), 2 * rows * v, 5 * rows * v,
+            {"rows": rows, "vocab": v, "top": top}, (1e-5, 1e-5))
+
+
+def _linear_logprobs(size):
+    import torch
+    from .. import ops
+    m, k, n = {"small": (64, 512, 4096), "decode": (32, 4096, 128256), "large": (2048, 4096, 128256)}[size]
+    x = torch.randn(m, k, device="cuda").bfloat16()
+    w = (torch.randn(n, k, device="cuda") * 2.5 / k ** 0.5).bfloat16()
+    ids = torch.randint(0, n, (m,), device="cuda", dtype=torch.int32)
+    lw = ops.LinearWeight("dense", w)
+
+    def run():
+        p = ops.linear_logprobs(x, lw, ids)
+        return torch.stack([p.logprob, p.entropy])
+
+    z = x.double() @ w.double().t() if size != "large" else None
+    want = None
+    if z is not None:
+        logp = torch.log_softmax(z, 1)
+        want = torch.stack([logp.gather(1, ids.long()[:, None])[:, 0], -(logp.exp() * logp).sum(1)])
+    return run, want, 2 * k * (m + n), 2 * m * n * k, {"m": m, "n": n, "k": k}, (1e-5, 1e-5)
+
+
+def _batch_plan(size):
+    import torch
+    from .. import ops
+    s, new, blocks = {"small": (8, 5, 64), "decode": (64, 1, 512), "large": (256, 200, 2048)}[size]
+    lens, starts = torch.full((s,), new, dtype=torch.int32), torch.arange(s, dtype=torch.int32) * 7
+    pages = torch.randperm(int(((starts + lens + 15) // 16).sum())).to(torch.int32)
+    got = [t.cuda() for t in (lens, starts, pages)]
+    flat = lambda p: torch.cat([f.reshape(-1).float() for f in p])
+    byts = 20 * s * new + 4 * s * blocks + 20 * s + 4 * pages.numel()
+    return ((lambda: flat(ops.batch_plan(*got, s * new, blocks))), flat(ops.batch_plan(lens, starts, pages, s * new, blocks)), byts, 0,
+            {"requests": s, "new": new, "blocks": blocks}, (0.0, 0.0))
+
+
 OPS = {"gemm-bf16": _gemm("bf16"), "gemm-fp8": _gemm("fp8"), "gemm-nvfp4": _gemm("nvfp4"), "gemm-mxfp4": _gemm("mxfp4"),
        "gemm-w4a4-nvfp4": _gemm_w4a4("nvfp4"), "gemm-w4a4-mxfp4": _gemm_w4a4("mxfp4"), "act-quant-fp4": _act_quant,
        "gated-delta-net": _gdn,
-       "rmsnorm": _rmsnorm, "gated-act": _gated, "argmax": _argmax, "paged-attention-fp8": _attention, "moe-route": _moe_route}
+       "rmsnorm": _rmsnorm, "gated-act": _gated, "argmax": _argmax, "paged-attention-fp8": _attention, "moe-route": _moe_route,
+       "token-logprobs": _token_logprobs, "linear-logprobs": _linear_logprobs, "batch-plan": _batch_plan}
 
 
 def run_op(op: str, size: str = "small") -> dict:

@@ -125,7 +125,7 @@ def _head(x: torch.Tensor, w: torch.Tensor, tokens: torch.Tensor, softcap: float
     tokens = tokens.contiguous()
     bn = 0 if r <= FEW_ROWS else core._prompt_tile(min(r, CHUNK_ROWS), n, False)
     floats = _k().sllm_head_logprobs_floats
-    step = max(256, min(CHUNK_ROWS, CHUNK_FLOATS // int(floats(1, n, bn))) // 256 * 256)
+    step = max(256, min(CHUNK_ROWS, CHUNK_FLOATS // max(1, int(floats(1, n, bn)))) // 256 * 256)
     ws = torch.empty(int(floats(min(r, step), n, bn)), dtype=torch.float32, device=dev)
     status = core.workspace(dev).status
     for lo in range(0, r, step):
@@ -135,7 +135,7 @@ def _head(x: torch.Tensor, w: torch.Tensor, tokens: torch.Tensor, softcap: float
                      entropy.data_ptr() + 4 * lo, status.data_ptr())
         _lib.check(rc, "head_logprobs")
         if _lib.audit_enabled():
-            _lib.record_dispatch("linear_logprobs", "head_logprobs_kernel", m=m, n=n, k=x.shape[1], bn=bn)
+            _lib.record_dispatch("linear_logprobs", "head_logprobs_kernel" if bn else "head_few_kernel", m=m, n=n, k=x.shape[1], bn=bn)
     return TokenLogprobs(lp, entropy)
 
 

@@ -265,9 +265,30 @@ def bench_prompt_kernels(reps):
         lambda: delta.general_delta(proj, spec, w2, *vecs, 1e-5, state, off, slot, False), reps), 0
 
 
+def bench_scoring(reps):
+    """(op, size, seconds, operations) of the ops around a scoring step, each through its public call."""
+    dev = "cuda"
+    i32 = lambda *shape, hi=1000: torch.randint(0, hi, shape, device=dev, dtype=torch.int32)
+    for s, new, cached, blocks in ((64, 1, 8000, 512), (300, 200, 100000, 8192), (1, 65536, 0, 4096)):
+        lens, starts = torch.full((s,), new, dtype=torch.int32, device=dev), i32(s, hi=cached + 1)
+        pages = torch.arange(int(((starts + lens + 15) // 16).sum()), dtype=torch.int32, device=dev)
+        yield "batch plan", f"{s} requests of {new}, table {blocks}", timed(lambda: ops.batch_plan(lens, starts, pages, s * new, blocks), reps), 0
+    for r, v, dtype, top in ((1, 128256, torch.bfloat16, 20), (64, 201088, torch.bfloat16, 5), (1500, 32768, torch.float16, 0),
+                             (4096, 128256, torch.bfloat16, 0), (4096, 128256, torch.bfloat16, 5), (4096, 128256, torch.bfloat16, 32)):
+        z = torch.randn(r, v, device=dev).to(dtype)
+        ids = i32(r)
+        yield "token log-probabilities", f"{r} x {v} {str(dtype)[6:]}, top {top}", timed(lambda: ops.token_logprobs(z, ids, top), reps), 5.0 * r * v
+        del z
+    for m, k, n, cap in ((1, 4096, 128256, 0.0), (48, 2880, 201088, 0.0), (777, 2560, 151936, 30.0), (4096, 4096, 128256, 0.0)):
+        x, w = torch.randn(m, k, device=dev).bfloat16(), LinearWeight("dense", (torch.randn(n, k, device=dev) * 2.5 / k ** 0.5).bfloat16())
+        ids = i32(m)
+        yield "head log-probabilities", f"{m} x {n} x {k}" + (f", cap {cap}" if cap else ""), timed(
+            lambda: ops.linear_logprobs(x, w, ids, softcap=cap), reps), 2.0 * m * n * k
+
+
 def main():
     ap = argparse.ArgumentParser()
-    ap.add_argument("--op", required=True, choices=["gemm", "gemm-w4", "attention", "prefill", "decode-gemms", "prompt-kernels"])
+    ap.add_argument("--op", required=True, choices=["gemm", "gemm-w4", "attention", "prefill", "decode-gemms", "prompt-kernels", "scoring"])
     ap.add_argument("--fmt", default="nvfp4", choices=["nvfp4", "mxfp4"])
     ap.add_argument("--groups", type=int, default=1)
     ap.add_argument("--active", type=int, default=0, help="gemm-w4, grouped: groups that receive tokens (0 = all)")
@@ -296,8 +317,8 @@ def main():
         print(json.dumps(bench_attention(a.batch, a.ctx, a.hq, a.hkv, a.hd, a.fp8, a.reps, a.graph)))
     elif a.op == "prefill":
         print(json.dumps(bench_prefill(a.seqs, a.len, a.hq, a.hkv, a.reps)))
-    elif a.op == "prompt-kernels":
-        for op, size, t, flops in bench_prompt_kernels(a.reps):
+    elif a.op in ("prompt-kernels", "scoring"):
+        for op, size, t, flops in (bench_prompt_kernels if a.op == "prompt-kernels" else bench_scoring)(a.reps):
             print(json.dumps({"op": op, "size": size, "us": round(t * 1e6, 1), **({"TFLOPs": round(flops / t / 1e12, 1)} if flops else {})}))
     else:
         for (n, k) in ((6144, 4096), (4096, 4096), (28672, 4096), (4096, 14336), (128256, 4096)):

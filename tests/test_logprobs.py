@@ -174,6 +174,48 @@ def test_the_head_launcher_refuses():
     assert f(*(ok[:3] + [129] + ok[4:8] + [0] + ok[9:])) == 1          # more rows than the kernel for few takes
 
 
+def test_rejected_launches_are_errors():
+    """Every entry's refusal reaches the caller, whichever path a call takes (a stand-in for the library counts them)."""
+    z, ids = torch.zeros(3, 8), torch.zeros(3, dtype=torch.int32)
+    x, w = torch.zeros((3, 8), dtype=torch.bfloat16), ops.LinearWeight("dense", torch.zeros((5, 8), dtype=torch.bfloat16))
+    i = lambda *v: torch.tensor(v, dtype=torch.int32)
+    for name, call in (("sllm_token_logprobs", lambda: ops.token_logprobs(z, ids, 2)), ("sllm_head_logprobs", lambda: ops.linear_logprobs(x, w, ids)),
+                       ("sllm_batch_plan", lambda: ops.batch_plan(i(1), i(0), i(0), 1, 1))):
+        fake = _lib.FakeKernelLibrary({name: [0, 5]})
+        _lib.install_fake(fake)
+        try:
+            call()
+            assert fake.count(name) == 1
+            with pytest.raises(_lib.KernelError):
+                call()
+        finally:
+            _lib.install_fake(None)
+
+
+def test_launches_go_to_the_device_of_their_tensors(monkeypatch):
+    """Two devices stood in for: the entry gets the stream that is current on the tensors' device, which is current while it runs."""
+    from sllm_b200.ops import core
+    now = [0]
+
+    class On:
+        def __init__(self, device):
+            self.index = device.index
+
+        def __enter__(self):
+            self.before, now[0] = now[0], self.index
+
+        def __exit__(self, *exc):
+            now[0] = self.before
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: now[0])
+    monkeypatch.setattr(torch.cuda, "device", On)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 100 + i, raising=False)
+    seen = []
+    for index in (0, 1):
+        assert core._launch(torch.device("cuda", index), lambda *a: seen.append((now[0], a)) or 0, 7) == 0
+    assert seen == [(0, (7, 100)), (1, (7, 101))] and now == [0]
+
+
 # ------------------------------------------------------------------------------------------ kernels
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])

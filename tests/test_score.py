@@ -12,6 +12,7 @@ from sllm_b200 import ops
 from sllm_b200.engine.batch import PageLists, make_prefill_batch
 from sllm_b200.engine.engine import Engine, build_engine
 from sllm_b200.models import config as MC
+from sllm_b200.ops import _lib
 
 DEV = "cuda"
 TEXTS = [[5, 9, 3, 7, 2, 8], [11], list(range(3, 60)), [4, 4]]
@@ -74,6 +75,20 @@ def test_score_on_cpu():
     assert eng.score([]) == [] and eng.cache.pool.stats()["sequences"] == 0
 
 
+def test_score_where_cpu_tensors_are_refused(monkeypatch):
+    """Nothing of the result's assembly on the host goes through an op (a server on a GPU refuses CPU tensors in ops)."""
+    eng = build_engine(MC.tiny_llama(), "cpu", num_pages=8, max_batch=2)
+    monkeypatch.setattr(eng, "_row_logprobs", lambda b, h, rows, tokens, top: ops.TokenLogprobs(
+        torch.zeros(rows.numel()), torch.zeros(rows.numel()), torch.zeros((rows.numel(), top), dtype=torch.int32), torch.zeros((rows.numel(), top))))
+    monkeypatch.setattr(eng.model, "hidden", lambda b, cache: None)
+    _lib.set_fail_closed(True)
+    try:
+        got = eng.score([[3], [1, 2, 3]], 2)
+    finally:
+        _lib.set_fail_closed(False)
+    assert got[0].logprob.shape == (0,) and got[0].top_ids.shape == (0, 2) and got[1].logprob.shape == (2,)
+
+
 def test_score_refusals_leave_nothing_behind():
     eng = build_engine(MC.tiny_llama(), "cpu", num_pages=4, max_batch=2)
     v = eng.cfg.vocab
@@ -98,7 +113,8 @@ def test_page_lists():
     assert pool.list_pages([a], [17]).tolist() == pool.pages(a)[:2] and pool.list_pages([], []).numel() == 0
     out = torch.full((2, 3), -1, dtype=torch.int32)
     assert pool.list_pages([a, b], [40, 1], out=out).tolist() == pool.pages(a) + pool.pages(b) and out[1].tolist()[1:] == [-1, -1]
-    for seqs, lens, o in (([a], [49], None), ([99], [1], None), ([a], [40], out[:1, :2].contiguous())):
+    for seqs, lens, o in (([a], [49], None), ([99], [1], None), ([a], [40], out[:1, :2].contiguous()), ([a], [17], out[0, :1].expand(9)),
+                          ([a], [17], out.long())):
         with pytest.raises(ValueError):
             pool.list_pages(seqs, lens, o)
 
