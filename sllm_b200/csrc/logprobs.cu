@@ -546,13 +546,19 @@ static cudaError_t logprobs_go(const LogprobParams& p, int cluster, cudaStream_t
                : launch_kernel_cluster(logprobs_kernel<T, kThreads, false, kLong>, grid, block, 0, st, cluster, 1u, p, cluster);
 }
 
-// us a launch that decide: many rows of up to kLpSmallUnits units go to CTAs of 64 threads (2655 x 6135 bf16: 9.5, with 256 threads 18.9), few
-// of them do not (138 x 2067 fp32 with 32 alternatives: 9.5 and 6.9).  Rows are shared by a cluster where they would not give every SM
-// four CTAs (100 x 128256 bf16 with 5 alternatives: 13.6 in clusters of four, 17.9 of eight; 300: 27.7 in clusters of two, 31.0 alone).
+// us a launch that decide.  Many rows: the shorter they are, the more of them an SM should have under way (2000 rows bf16 of 6000, 12000 and 50000
+// with CTAs of 64, 128 and 256 threads: 8.5 / 9.7 / 13.3, 13.7 / 12.5 / 18.3, 45.5 / 40.1 / 42.6); longer rows take 128 threads only where the last wave
+// of CTAs is filled as well as with 256 (700 x 50000: 25.3 and 20.0; 1500 x 32768: 24.3 and 23.4).  Few rows do not (138 x 2067 fp32 with 32
+// alternatives: 9.5 with 64 threads, 6.9 with 256): they are shared by a cluster where they would not give every SM four CTAs (100 x 128256 bf16
+// with 5 alternatives: 13.6 in clusters of four, 17.9 of eight; 300: 27.7 in clusters of two, 31.0 alone).
 template <typename T>
 static cudaError_t logprobs_go(const LogprobParams& p, cudaStream_t st) {
   const long long units = (static_cast<long long>(p.vocab) + LpVec<T>::kN - 1) / LpVec<T>::kN;
   if (units <= 256 || (units <= kLpSmallUnits && p.rows > kLpFill)) return logprobs_go<T, 64>(p, 1, st);
+  if (p.rows > kLpFill && units <= 8 * kLpSmallUnits) {
+    const long long wide = (p.rows + 591LL) / 592 * 592, narrow = (p.rows + 1183LL) / 1184 * 1184;      // rows that the waves would hold
+    if (units <= 2 * kLpSmallUnits || (p.rows > 1184 && narrow <= wide)) return logprobs_go<T, 128>(p, 1, st);
+  }
   if (p.rows >= kLpLongRows && units >= 32 * 256) return logprobs_go<T, 256, true>(p, 1, st);
   int cluster = 1;
   while (cluster < kLpMaxCluster && static_cast<long long>(p.rows) * cluster * 2 <= kLpFill && units >= 2 * cluster * 256) cluster *= 2;
