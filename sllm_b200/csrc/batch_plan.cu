@@ -4,8 +4,11 @@
 // slot pages[first[i] + position / page] * page + position % page; the table's row i holds the request's pages, then zeros.  Rows
 // behind the last request: position, request and slot -1, no keys.  A request without new tokens has no last row (-1).
 //
-// One launch: every CTA takes the running sums of all requests into shared memory (loads out of L2, all at once) and then its share of the rows and of the table, so that neither a long request nor a wide table waits for one CTA.  A second launch
-// for the sums would cost more than they do (2.4 us a launch at 64 requests).
+// One launch: every CTA takes the running sums of all requests into shared memory (loads out of L2, all at once) and then its share
+// of the rows and of the table, so that neither a long request nor a wide table waits for one CTA.  A second launch for the sums would
+// cost more than they do (2.4 us a launch at 64 requests).  Measured (us a launch, in brackets its bytes at the copy bandwidth): 64
+// requests of one token 3.2 (0.03), one of 65536 tokens 3.4 (0.2), 300 with a table of 8192 columns 8.5 (2.2), 16384 requests 71 (0.3; 128 KB of
+// sums hold one CTA per SM).
 #include <climits>
 #include "common.cuh"
 #include "api.h"
