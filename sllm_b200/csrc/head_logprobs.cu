@@ -579,11 +579,12 @@ SLLM_EXPORT long long sllm_head_logprobs_floats(int m, int n, int bn) {
   return m * (4 * head_parts(n, bn) + 1);
 }
 
-// x [m, k] bf16 (row stride ldx elements), w [n, k] bf16 contiguous, tokens [m]; logprob and entropy [m].  cap > 0: soft cap.  bn: columns
+// x [m, k] bf16 (row stride ldx elements), w [n, k] bf16 contiguous, tokens [m]; logprob and entropy [m].  cap: soft cap (1e-30 to 1e30), or 0.  bn: columns
 // of a CTA pair's tile, 128 or 256; 0: the kernel for up to 128 rows.  k a multiple of 8, rows of x multiples of 16 bytes.
 SLLM_EXPORT int sllm_head_logprobs(const void* x, const void* w, const int* tokens, int m, int n, int k, long long ldx, float cap, int bn,
                                    float* ws, long long ws_floats, float* logprob, float* entropy, int* status, void* stream) {
-  if (!x || !w || !tokens || !ws || !logprob || !entropy || m <= 0 || n <= 0 || k <= 0 || ldx < k || !(cap >= 0.f && cap < INFINITY))
+  if (!x || !w || !tokens || !ws || !logprob || !entropy || m <= 0 || n <= 0 || k <= 0 || ldx < k ||
+      !(cap == 0.f || (cap >= 1e-30f && cap <= 1e30f)))
     return SLLM_ERR_INVALID_ARGUMENT;
   if ((bn != 0 && bn != 128 && bn != 256) || (bn == 0 && m > kHlRows)) return SLLM_ERR_INVALID_ARGUMENT;
   if (m > (1 << 24) || n > (1 << 30) || k > (1 << 24)) return SLLM_ERR_LIMIT;

@@ -19,6 +19,7 @@ _SIGS = {
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 MAX_TOP = 32
 MAX_VOCAB = 1 << 30
+MIN_CAP, MAX_CAP = 1e-30, 1e30 # whose reciprocals are normal numbers
 CHUNK_ROWS = 1 << 15
 FEW_ROWS = 128                 # up to here a row's tile is shared by no CTA pair (csrc/head_logprobs.cu)
 CHUNK_LOGITS = 1 << 26         # logits that `linear_logprobs` holds at a time where it writes them,
@@ -147,8 +148,10 @@ def linear_logprobs(x, w, tokens: torch.Tensor, softcap: float = 0.0, top: int =
     xd = x.data if isinstance(x, core.QTensor) else x
     if xd.dim() != 2 or xd.shape[1] != w.in_features:
         raise ValueError("x is [rows, in_features]")
-    if not 0.0 <= softcap < float("inf"):
-        raise ValueError("the soft cap is finite and positive, or 0 for none")
+    if w.kind != "w4" and w.w.device != xd.device:
+        raise ValueError("rows and weight are on one device")
+    if softcap != 0.0 and not MIN_CAP <= softcap <= MAX_CAP:
+        raise ValueError(f"the soft cap lies between {MIN_CAP} and {MAX_CAP}, or is 0 for none")
     if not 0 <= top <= MAX_TOP:
         raise ValueError(f"top lies between 0 and {MAX_TOP}")
     _check_tokens(tokens, xd.shape[0], xd.device)

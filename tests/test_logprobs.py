@@ -139,7 +139,10 @@ def test_refusals():
                 lambda: ops.token_logprobs(z, ids, -1), lambda: ops.token_logprobs(z, ids, 33),
                 lambda: ops.token_logprobs(z, ids.view(3, 1, 1)), lambda: ops.linear_logprobs(torch.zeros(3, 5), w, ids),
                 lambda: ops.linear_logprobs(torch.zeros(3, 4), w, ids.view(3, 1)), lambda: ops.linear_logprobs(torch.zeros(3, 4), w, ids, softcap=-1.0),
-                lambda: ops.linear_logprobs(torch.zeros(3, 4), w, ids, softcap=NAN), lambda: ops.linear_logprobs(torch.zeros(3, 4), w, ids, top=40)):
+                lambda: ops.linear_logprobs(torch.zeros(3, 4), w, ids, softcap=NAN), lambda: ops.linear_logprobs(torch.zeros(3, 4), w, ids, softcap=1e31),
+                lambda: ops.linear_logprobs(torch.zeros(3, 4), w, ids, softcap=INF), lambda: ops.linear_logprobs(torch.zeros(3, 4), w, ids, softcap=1e-40),
+                lambda: ops.linear_logprobs(torch.zeros(3, 4), ops.LinearWeight("dense", torch.zeros((8, 4), device="meta")), ids),
+                lambda: ops.linear_logprobs(torch.zeros(3, 4), w, ids, top=40)):
         with pytest.raises(ValueError):
             bad()
 
@@ -165,7 +168,7 @@ def test_the_head_launcher_refuses():
         assert floats(0, 8, bn) == 0 and floats(5, 70000, bn) % 5 == 0
     assert floats(5, 8, 64) == 0 and floats(5, (1 << 30) + 1, 0) == 0
     ok = [256, 256, 256, 100, 1000, 64, 64, 0.0, 256, 256, 1 << 20, 256, 256, 256, None]
-    for at, value, code in ((0, None, 1), (1, None, 1), (2, None, 1), (3, 0, 1), (4, 0, 1), (5, 0, 1), (6, 63, 1), (7, -1.0, 1), (7, NAN, 1), (7, INF, 1),
+    for at, value, code in ((0, None, 1), (1, None, 1), (2, None, 1), (3, 0, 1), (4, 0, 1), (5, 0, 1), (6, 63, 1), (7, -1.0, 1), (7, NAN, 1), (7, INF, 1), (7, 1e-40, 1),
                             (8, 64, 1), (9, None, 1), (11, None, 1), (12, None, 1), (3, (1 << 24) + 1, 7), (4, (1 << 30) + 1, 7), (6, 68, 3), (0, 264, 3),
                             (1, 264, 3), (9, 264, 3), (10, floats(100, 1000, 256) - 1, 4)):
         a = list(ok)
@@ -373,6 +376,16 @@ HEADS = [(1, 8, 1), (1, 64, 300), (3, 72, 1000), (16, 512, 2048), (17, 128, 777)
 def test_head_matches_the_definition(r, d, v, cap):
     x, w, ids = head_case(r, d, v, r + d + v)
     head_check(x, w, ids, cap, ops.linear_logprobs(x, ops.LinearWeight("dense", w), ids, softcap=cap))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cap", [1e-20, 0.5, 3.0, 1e25])
+@pytest.mark.parametrize("r", [6, 150])
+def test_head_with_caps_of_any_size(r, cap):
+    """Logits far below the cap, about it and far beyond: the polynomial, both forms in one group of columns, and saturation."""
+    x, w, ids = head_case(r, 64, 700, 11)
+    head_check(x, w, ids, cap, ops.linear_logprobs(x, ops.LinearWeight("dense", w), ids, softcap=cap)) if cap < 1e3 else \
+        head_check(x, w, ids, 0.0, ops.linear_logprobs(x, ops.LinearWeight("dense", w), ids, softcap=cap))     # (tanh(u) = u to 2^-24 there)
 
 
 @pytest.mark.gpu
