@@ -16,7 +16,7 @@
 // A tile's sum over K is taken in chains of kHlChain K blocks with an accumulator of their own, which the epilogue warps add in fp32
 // registers while the next chain is multiplied: tensor memory rounds towards zero, and a chain's error grows with its length (4096 wide:
 // 2.3e-7 of the log-probabilities with chains of 8, 4.6e-7 with 16, 9.7e-7 with 32, which takes 1 % less time).
-#include <cfloat>
+#include <atomic>
 #include "pair_mma.cuh"
 #include "api.h"
 #include "tmap.h"
@@ -518,6 +518,17 @@ static int head_join(const HlParams& p, int parts, float* logprob, float* entrop
              : SLLM_ERR_CUDA;
 }
 
+// Allows a kernel its shared memory, once per device (a bit of `known` each).
+static bool head_shared_memory(const void* kernel, size_t bytes, std::atomic<uint64_t>& known) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+  if (known.load(std::memory_order_relaxed) & bit) return true;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)) != cudaSuccess) return false;
+  known.fetch_or(bit, std::memory_order_relaxed);
+  return true;
+}
+
 template <int BN>
 static int head_logprobs_go(const void* x, const void* w, int k, long long ldx, HlParams& p, float* logprob, float* entropy, cudaStream_t st) {
   using S = HlShape<BN>;
@@ -528,8 +539,8 @@ static int head_logprobs_go(const void* x, const void* w, int k, long long ldx, 
   p.tiles_m = (p.m + 255) / 256;
   p.tiles_n = (p.n + BN - 1) / BN;
   const size_t smem = S::kStages * S::kStage + sizeof(HlShared) + 1024;
-  if (cudaFuncSetAttribute(head_logprobs_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess)
-    return SLLM_ERR_CUDA;
+  static std::atomic<uint64_t> known{0};
+  if (!head_shared_memory(reinterpret_cast<const void*>(head_logprobs_kernel<BN>), smem, known)) return SLLM_ERR_CUDA;
   const long long tiles = static_cast<long long>(p.tiles_m) * p.tiles_n;
   if (tiles * p.num_kb > 0x7fffffffLL) return SLLM_ERR_LIMIT;
   const int pairs = tiles < 74 ? static_cast<int>(tiles) : 74;
@@ -555,8 +566,8 @@ static int head_few_go(const void* x, const void* w, int k, long long ldx, HlPar
   head_few_shape(p.n, ctas, share);
   if ((share / kHfTile + 1LL) * p.num_kb > 0x7fffffffLL) return SLLM_ERR_LIMIT;
   const size_t smem = kHfStages * kHfStage + sizeof(HlShared) + 1024;
-  if (cudaFuncSetAttribute(head_few_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess)
-    return SLLM_ERR_CUDA;
+  static std::atomic<uint64_t> known{0};
+  if (!head_shared_memory(reinterpret_cast<const void*>(head_few_kernel), smem, known)) return SLLM_ERR_CUDA;
   if (launch_kernel(head_few_kernel, dim3(ctas), dim3(kHlThreads), smem, st, 1u, tx, tw, p, share, x_rows) != cudaSuccess) return SLLM_ERR_CUDA;
   return head_join(p, 2 * ctas, logprob, entropy, st);
 }

@@ -115,8 +115,8 @@ def _head(x: torch.Tensor, w: torch.Tensor, tokens: torch.Tensor, softcap: float
     """bf16 rows against a dense matrix on the tensor cores, without logits in memory."""
     from . import core
     r, n, dev = x.shape[0], w.shape[0], x.device
-    out = torch.empty((2, r), dtype=torch.float32, device=dev)
-    lp, entropy = out.unbind()
+    out = torch.empty(2 * r, dtype=torch.float32, device=dev)
+    lp, entropy = out.as_strided((r,), (1,), 0), out.as_strided((r,), (1,), r)
     if not r:
         return TokenLogprobs(lp, entropy)
     if x.stride(1) != 1 or x.stride(0) % 8 or x.stride(0) < x.shape[1] or x.data_ptr() % 16:      # (a TMA copy needs rows of whole 16 bytes)
@@ -125,9 +125,9 @@ def _head(x: torch.Tensor, w: torch.Tensor, tokens: torch.Tensor, softcap: float
         tokens = tokens.clamp(-1, n).to(torch.int32)
     tokens = tokens.contiguous()
     bn = 0 if r <= FEW_ROWS else core._prompt_tile(min(r, CHUNK_ROWS), n, False)
-    floats = _k().sllm_head_logprobs_floats
-    step = max(256, min(CHUNK_ROWS, CHUNK_FLOATS // max(1, int(floats(1, n, bn)))) // 256 * 256)
-    ws = torch.empty(int(floats(min(r, step), n, bn)), dtype=torch.float32, device=dev)
+    per_row = int(_k().sllm_head_logprobs_floats(1, n, bn))
+    step = max(256, min(CHUNK_ROWS, CHUNK_FLOATS // max(1, per_row)) // 256 * 256)
+    ws = torch.empty(per_row * min(r, step), dtype=torch.float32, device=dev)
     status = core.workspace(dev).status
     for lo in range(0, r, step):
         m = min(step, r - lo)

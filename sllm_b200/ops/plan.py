@@ -58,10 +58,10 @@ def batch_plan(new_lens: torch.Tensor, starts: torch.Tensor, pages: torch.Tensor
     batch, the sum of new_lens or more (a captured step's padding).  ``table`` (int32 [S, max_blocks], any row stride) receives
     the block table in place of a new tensor.  A length below 0 counts as 0; entries whose page lies beyond the list read page 0, and
     a table narrower than a request holds its first pages.  Positions stay below 2^31, requests at 16384 or less."""
-    for t in (new_lens, starts, pages):
-        if t.dtype != torch.int32 or t.dim() != 1 or t.device != new_lens.device or not t.is_contiguous():
-            raise ValueError("lengths, starts and pages are contiguous int32 vectors on one device")
     s, dev = new_lens.numel(), new_lens.device
+    for t in (new_lens, starts, pages):
+        if t.dtype is not torch.int32 or t.dim() != 1 or t.device != dev or not t.is_contiguous():
+            raise ValueError("lengths, starts and pages are contiguous int32 vectors on one device")
     if starts.numel() != s:
         raise ValueError("one start per length")
     if s > MAX_REQUESTS:
@@ -74,15 +74,22 @@ def batch_plan(new_lens: torch.Tensor, starts: torch.Tensor, pages: torch.Tensor
     if _lib.on_cpu(new_lens):
         return _cpu(new_lens, starts, pages, rows, max_blocks, page_size,
                     torch.empty((s, max_blocks), dtype=torch.int32) if table is None else table)
-    # (one allocation: a tensor of its own for each part costs more than the kernel)
-    cells = 0 if table is not None else s * max_blocks
-    ca, sa, ra, la = -cells % 4, -(s + 1) % 4, -rows % 4, -rows % 2      # (every part starts at 16 bytes)
-    half = (cells + ca + s + 1 + sa + 3 * (rows + ra)) // 2
-    rest, slots, _, last_rows = torch.empty(half + rows + la + s, dtype=torch.int64, device=dev).split_with_sizes((half, rows, la, s))
-    own, _, row_off, _, positions, _, seq_index, _, kv_lens, _ = rest.view(torch.int32).split_with_sizes(
-        (cells, ca, s + 1, sa, rows, ra, rows, ra, rows, ra))
+    # (one allocation, every part of it at a multiple of 16 bytes: a tensor of its own for each costs more than the kernel)
+    row4 = (rows + 3) & -4
+    off_at = 0 if table is not None else (s * max_blocks + 3) & -4
+    pos_at = off_at + ((s + 4) & -4)
+    slot_at = (pos_at + 3 * row4) // 2
+    last_at = slot_at + ((rows + 1) & -2)
+    out64 = torch.empty(last_at + s, dtype=torch.int64, device=dev)
+    out = out64.view(torch.int32)
     if table is None:
-        table = own.view(s, max_blocks)
+        table = out.as_strided((s, max_blocks), (max_blocks, 1), 0)
+    row_off = out.as_strided((s + 1,), (1,), off_at)
+    positions = out.as_strided((rows,), (1,), pos_at)
+    seq_index = out.as_strided((rows,), (1,), pos_at + row4)
+    kv_lens = out.as_strided((rows,), (1,), pos_at + 2 * row4)
+    slots = out64.as_strided((rows,), (1,), slot_at)
+    last_rows = out64.as_strided((s,), (1,), last_at)
     rc = _launch(dev, _k().sllm_batch_plan, new_lens.data_ptr(), starts.data_ptr(), pages.data_ptr(), pages.numel(), s, rows, max_blocks,
                  table.stride(0) if s > 1 else max_blocks, page_size, row_off.data_ptr(), positions.data_ptr(), seq_index.data_ptr(),
                  kv_lens.data_ptr(), slots.data_ptr(), last_rows.data_ptr(), table.data_ptr())
