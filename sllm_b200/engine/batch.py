@@ -54,6 +54,15 @@ class PageLists:
     max_blocks: int
     page_size: int
 
+    def table(self, lengths: list) -> torch.Tensor:
+        """The block table on the host, for sequences of these lengths."""
+        out, at = torch.zeros((len(lengths), self.max_blocks), dtype=torch.int32), 0
+        for row, n in zip(out, lengths):
+            used = (n + self.page_size - 1) // self.page_size
+            row[:used] = self.pages[at:at + used]
+            at += used
+        return out
+
 
 def _planned_batch(prompts: list, table: Union[torch.Tensor, PageLists, None], device, starts: list, last_only: bool) -> ForwardBatch:
     """`make_prefill_batch` on a GPU: one copy of tokens, lengths and pages, and one launch for everything that follows from them
@@ -84,10 +93,13 @@ def _planned_batch(prompts: list, table: Union[torch.Tensor, PageLists, None], d
 
 def make_prefill_batch(prompts: list, block_table: Union[torch.Tensor, PageLists, None], device, start_positions: Optional[list] = None,
                        last_only: bool = True) -> ForwardBatch:
-    """prompts: list of token-id lists, one per row of block_table (on a GPU also `PageLists` in its place)."""
+    """prompts: list of token-id lists, one per row of block_table (or `PageLists` in its place)."""
     from ..ops.plan import MAX_REQUESTS
     if torch.device(device).type == "cuda" and len(prompts) <= MAX_REQUESTS:
         return _planned_batch(prompts, block_table, device, list(start_positions) if start_positions is not None else [0] * len(prompts), last_only)
+    if isinstance(block_table, PageLists):
+        begun = start_positions or [0] * len(prompts)
+        block_table = block_table.table([a + len(p) for a, p in zip(begun, prompts)]).to(device)
     toks, pos, sidx = [], [], []
     cu = [0]
     rows = []

@@ -119,6 +119,14 @@ def test_page_lists():
             pool.list_pages(seqs, lens, o)
 
 
+def test_batches_from_page_lists_on_the_host():
+    pages = torch.tensor([7, 3, 9, 4], dtype=torch.int32)
+    b = make_prefill_batch([[1] * 20, [2]], PageLists(pages, 3, 16), "cpu")
+    assert b.block_table.tolist() == [[7, 3, 0], [9, 0, 0]]
+    b = make_prefill_batch([[1], [2] * 3], PageLists(pages, 3, 16), "cpu", [16, 29])
+    assert b.block_table.tolist() == [[7, 3, 0], [9, 4, 0]] and b.kv_lens.tolist() == [17, 30, 31, 32]
+
+
 def test_score_runner(tmp_path, capsys):
     from sllm_b200.cli import convert
     from sllm_b200.evidence import score
