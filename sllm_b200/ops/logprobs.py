@@ -7,7 +7,7 @@ from typing import NamedTuple, Optional
 
 import torch
 
-from . import _lib
+from . import _lib, core
 from .core import _launch
 
 P, I, L = C.c_void_p, C.c_int, C.c_longlong
@@ -111,9 +111,20 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     return TokenLogprobs(lp, entropy, ids, tlp)
 
 
+_head_sizes: dict = {}         # (n, bn) -> floats of workspace per row
+
+
+def _head_floats(n: int, bn: int) -> int:
+    floats = _head_sizes.get((n, bn))
+    if floats is None:
+        floats = int(_k().sllm_head_logprobs_floats(1, n, bn))
+        if floats and len(_head_sizes) < 256:        # (0: a stand-in for the library)
+            _head_sizes[n, bn] = floats
+    return floats
+
+
 def _head(x: torch.Tensor, w: torch.Tensor, tokens: torch.Tensor, softcap: float) -> TokenLogprobs:
     """bf16 rows against a dense matrix on the tensor cores, without logits in memory."""
-    from . import core
     r, n, dev = x.shape[0], w.shape[0], x.device
     out = torch.empty(2 * r, dtype=torch.float32, device=dev)
     lp, entropy = out.as_strided((r,), (1,), 0), out.as_strided((r,), (1,), r)
@@ -125,7 +136,7 @@ def _head(x: torch.Tensor, w: torch.Tensor, tokens: torch.Tensor, softcap: float
         tokens = tokens.clamp(-1, n).to(torch.int32)
     tokens = tokens.contiguous()
     bn = 0 if r <= FEW_ROWS else core._prompt_tile(min(r, CHUNK_ROWS), n, False)
-    per_row = int(_k().sllm_head_logprobs_floats(1, n, bn))
+    per_row = _head_floats(n, bn)
     step = max(256, min(CHUNK_ROWS, CHUNK_FLOATS // max(1, per_row)) // 256 * 256)
     ws = torch.empty(per_row * min(r, step), dtype=torch.float32, device=dev)
     status = core.workspace(dev).status
@@ -144,7 +155,6 @@ def linear_logprobs(x, w, tokens: torch.Tensor, softcap: float = 0.0, top: int =
     """`token_logprobs` of the logits x W^T (``softcap`` > 0: softcap * tanh(logit / softcap)) for one token per row, in memory that
     does not grow with rows * vocabulary.  ``x``: hidden rows [R, d] as `ops.linear` takes them for ``w``; ``tokens`` [R].  Logits of
     dense weights are not rounded on the way (those of FP8 and 4-bit weights are bf16)."""
-    from . import core
     xd = x.data if isinstance(x, core.QTensor) else x
     if xd.dim() != 2 or xd.shape[1] != w.in_features:
         raise ValueError("x is [rows, in_features]")
