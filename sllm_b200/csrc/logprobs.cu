@@ -4,6 +4,7 @@
 // Alternatives are ordered by logit, equal ones by id.  -inf shuts a token out; a row of nothing else has log p = -inf, H = 0 and
 // no alternatives (id -1).  With +inf logits the row is uniform over them; a NaN makes the row's numbers NaN and leaves no
 // alternatives.  A given id below 0 stands for no token (0), one beyond the vocabulary has log p NaN.
+#include <algorithm>
 #include <cfloat>
 #include <type_traits>
 #include "pair_mma.cuh"
@@ -154,7 +155,7 @@ constexpr float kLpSlack = 4.f;            // a thread's sums are taken anew whe
 
 constexpr int kLpMaxCluster = 8;
 constexpr int kLpSmallUnits = 1024;
-constexpr int kLpFill = 640;                // CTAs of 256 threads from which a row has one of its own (the card holds 592)
+constexpr int kLpFill = 592;                // CTAs of 256 threads that the card holds; of 128 threads twice as many
 constexpr int kLpLongRows = 2368;
 constexpr int kLpMaxVocab = 1 << 30;       // ids and units stay below 2^31
 
@@ -552,20 +553,22 @@ static cudaError_t logprobs_go(const LogprobParams& p, int cluster, cudaStream_t
 // us a launch that decide.  Many rows: the shorter they are, the more of them an SM should have under way (2000 rows bf16 of 6000, 12000 and 50000
 // with CTAs of 64, 128 and 256 threads: 8.5 / 9.7 / 13.3, 13.7 / 12.5 / 18.3, 45.5 / 40.1 / 42.6); longer rows take 128 threads only where the last wave
 // of CTAs is filled as well as with 256 (700 x 50000: 25.3 and 20.0; 1500 x 32768: 24.3 and 23.4).  Few rows do not (138 x 2067 fp32 with 32
-// alternatives: 9.5 with 64 threads, 6.9 with 256): they are shared by a cluster where they would not give every SM four CTAs (100 x 128256 bf16
-// with 5 alternatives: 13.6 in clusters of four, 17.9 of eight; 300: 27.7 in clusters of two, 31.0 alone).
+// alternatives: 9.5 with 64 threads, 6.9 with 256): a cluster shares a row, as many CTAs as the card holds at a time and no more (with 5 alternatives
+// bf16: 80 x 128256 13.7 in clusters of eight with 128 threads, 16.5 with 256, which do not fit; 160 x 128256 17.0 in threes, 20.2 in fours; 300 x 32000
+// 11.7 alone, 15.4 in twos; one row 7 in a cluster of eight).
 template <typename T>
 static cudaError_t logprobs_go(const LogprobParams& p, cudaStream_t st) {
   const long long units = (static_cast<long long>(p.vocab) + LpVec<T>::kN - 1) / LpVec<T>::kN;
   if (units <= 256 || (units <= kLpSmallUnits && p.rows > kLpFill)) return logprobs_go<T, 64>(p, 1, st);
   if (p.rows > kLpFill && units <= 8 * kLpSmallUnits) {
-    const long long wide = (p.rows + 591LL) / 592 * 592, narrow = (p.rows + 1183LL) / 1184 * 1184;      // rows that the waves would hold
-    if (units <= 2 * kLpSmallUnits || (p.rows > 1184 && narrow <= wide)) return logprobs_go<T, 128>(p, 1, st);
+    const long long of256 = (p.rows + 591LL) / 592 * 592, of128 = (p.rows + 1183LL) / 1184 * 1184;      // rows that the waves would hold
+    if (units <= 2 * kLpSmallUnits || (p.rows > 1184 && of128 <= of256)) return logprobs_go<T, 128>(p, 1, st);
   }
   if (p.rows >= kLpLongRows && units >= 32 * 256) return logprobs_go<T, 256, true>(p, 1, st);
-  int cluster = 1;
-  while (cluster < kLpMaxCluster && static_cast<long long>(p.rows) * cluster * 2 <= kLpFill && units >= 2 * cluster * 256) cluster *= 2;
-  return logprobs_go<T, 256>(p, cluster, st);
+  const bool narrow = p.rows > kLpFill / kLpMaxCluster && p.rows <= 2 * kLpFill / kLpMaxCluster;
+  const long long fits = units / (narrow ? 256 : 512);         // (two units a thread at least)
+  const int wanted = narrow ? kLpMaxCluster : static_cast<int>(kLpFill / p.rows), cluster = static_cast<int>(std::min<long long>(std::min(wanted, kLpMaxCluster), fits));
+  return narrow && cluster > 1 ? logprobs_go<T, 128>(p, cluster, st) : logprobs_go<T, 256>(p, cluster > 1 ? cluster : 1, st);
 }
 
 }  // namespace sllm

@@ -225,7 +225,8 @@ def test_launches_go_to_the_device_of_their_tensors(monkeypatch):
 @pytest.mark.parametrize("r,v,gap,shift,top", [(1, 1, 0, 0, 3), (2, 5, 3, 1, 2), (3, 31, 0, 0, 32), (5, 257, 1, 1, 1), (4, 2048, 0, 0, 5),
                                                (7, 4099, 5, 3, 20), (1, 32000, 0, 0, 32), (300, 1000, 24, 8, 4), (700, 515, 0, 1, 0), (2, 131077, 11, 7, 20),
                                                (160, 9001, 0, 0, 7), (650, 9001, 5, 3, 6), (1250, 8400, 0, 0, 0), (593, 12289, 7, 1, 32),
-                                               (700, 12289, 7, 1, 32), (2000, 16500, 1, 3, 5)])
+                                               (700, 12289, 7, 1, 32), (2000, 16500, 1, 3, 5), (80, 40001, 3, 5, 5), (100, 17000, 0, 0, 32),
+                                               (148, 70000, 1, 1, 3), (160, 33001, 0, 2, 32), (197, 20000, 0, 0, 4), (118, 20011, 0, 0, 20), (30, 60000, 5, 0, 32)])
 def test_kernel_matches_the_definition(dtype, r, v, gap, shift, top):
     z, ids = rows(r, v, dtype, r * v, gap, shift, device=DEV)
     check(z, ids, top, ops.token_logprobs(z, ids.int() if r % 2 else ids, top))
