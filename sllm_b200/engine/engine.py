@@ -302,7 +302,7 @@ class Engine:
                 x = ops.rmsnorm(h.index_select(0, rows), m.w.final_norm, cfg.rms_eps, cfg.norm_offset_one)
             capped = cfg.family in ("llama", "gemma4", "sepedra")          # families whose logits pass the soft cap
             return ops.linear_logprobs(x, m.w.lm_head, tokens, softcap=cfg.logit_softcap if capped else 0.0)
-        parts, step = [], max(1, ops.logprobs.CHUNK_LOGITS // cfg.vocab)
+        parts, step = [], ops.logprobs.chunk_rows(cfg.vocab)
         for lo in range(0, rows.numel(), step):
             b.logit_rows = rows[lo:lo + step]
             z = m.logits(h, b)

@@ -20,10 +20,10 @@ _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 MAX_TOP = 32
 MAX_VOCAB = 1 << 30
 MIN_CAP, MAX_CAP = 1e-30, 1e30 # whose reciprocals are normal numbers
-CHUNK_ROWS = 1 << 15
 FEW_ROWS = 128                 # up to here a row's tile is shared by no CTA pair (csrc/head_logprobs.cu)
-CHUNK_LOGITS = 1 << 26         # logits that `linear_logprobs` holds at a time where it writes them,
-CHUNK_FLOATS = 1 << 25         # floats of its workspace where it does not (a sixteenth of the logits' number)
+CHUNK_LOGITS = 1 << 27         # logits that `linear_logprobs` holds at a time where it writes them
+CHUNK_FLOATS = 1 << 25         # floats of its workspace where it does not (a thirty-second of the logits' number, with narrow tiles a sixteenth),
+CHUNK_ROWS = 1 << 15           # and rows of a launch
 
 
 _lib.EXTRA_KERNEL_SIGNATURES.update(_SIGS)
@@ -37,6 +37,12 @@ class TokenLogprobs(NamedTuple):
     entropy: torch.Tensor                          # [R]
     top_ids: Optional[torch.Tensor] = None         # int32
     top_logprobs: Optional[torch.Tensor] = None
+
+
+def chunk_rows(vocab: int) -> int:
+    """Rows whose logits are written at a time: whole tiles of 256 where there are that many."""
+    rows = max(1, CHUNK_LOGITS // vocab)
+    return rows // 256 * 256 or rows
 
 
 def _check_tokens(tokens: torch.Tensor, rows: int, device) -> None:
@@ -170,7 +176,7 @@ def linear_logprobs(x, w, tokens: torch.Tensor, softcap: float = 0.0, top: int =
     if (not top and w.kind == "dense" and not _lib.on_cpu(xd) and xd.dtype == w.w.dtype == torch.bfloat16 and w.in_features % 8 == 0
             and w.w.is_contiguous() and w.w.data_ptr() % 16 == 0):
         return _head(xd, w.w, tokens, softcap)
-    step = max(1, CHUNK_LOGITS // w.out_features)
+    step = chunk_rows(w.out_features)
     parts = []
     for lo in range(0, xd.shape[0], step):
         hi = min(lo + step, xd.shape[0])
