@@ -125,3 +125,29 @@ def test_captured_plan_follows_its_inputs():
             t.copy_(v)
         g.replay()
         same(got, walk(c[0], c[1], c[2], 16, 4, 16))
+
+
+@pytest.mark.gpu
+def test_calls_from_two_threads():
+    import threading
+    cases = [case(lens(9000, 2, 13), lens(9000, 9, 14), 4), case(lens(16384, 2, 15), lens(16384, 9, 16), 4)]
+    want = [walk(*c, sum(c[0]), 4, 4) for c in cases]
+    held = [tensors(*c, DEV) for c in cases]
+    torch.cuda.synchronize()
+    failed = []
+
+    def run(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(200):
+                    got = ops.batch_plan(*held[i], sum(cases[i][0]), 4, 4)
+                torch.cuda.current_stream().synchronize()
+                same(got, want[i])
+        except BaseException as e:
+            failed.append(e)
+    threads = [threading.Thread(target=run, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
