@@ -68,18 +68,25 @@ __device__ __forceinline__ float2 lp_pair(const LpVec<T>& v, int i) {
 }
 
 // Sums are taken in powers of two, t = z log2(e) - m2 with m2 the rounded product of the reference: S = sum 2^t and W = sum 2^t t.
-// Logits below kLow (-inf and masks of the type's lowest value) count as it, so that 2^t t is 0 and no NaN; where a row's largest
-// logit is not well above it, or beyond kHigh, the sums are taken anew from exact differences (`lp_wide`).
+// Rounding moves m2 by up to half a unit in its last place (`lp_rest`), and 2^t of the largest logit is 2 to as much: between 1/2 and 2 below
+// 2^24, but 0 or infinite from 1e10 on.  So logits below kLow count as it (-inf too, whose 2^t t would be NaN), and where a range's
+// largest logit is not well above kLow, or beyond kHigh, its sums are taken anew from exact differences (`lp_wide`): the range is read
+// twice (4096 x 128256 bf16 about 1e8: 514 us, 184 of ordinary logits; one such row 6.9 and 3.7).
 template <typename T>
 struct LpRange {
   static constexpr bool kHalf = std::is_same_v<T, __half>;
-  static constexpr float kLow = kHalf ? -60000.f : -7.9228163e28f;      // (-2^96)
-  static constexpr float kWide = kHalf ? -59000.f : -3.9614081e28f;     // (-2^95)
-  static constexpr float kHigh = 3.9614081e28f;
-  static constexpr uint32_t kLowPair = kHalf ? 0xfb53fb53u : 0xef80ef80u;
+  static constexpr float kLow = kHalf ? -60000.f : -16777216.f;         // (-2^24)
+  static constexpr float kWide = kHalf ? -59000.f : -8388608.f;         // (-2^23)
+  static constexpr float kHigh = 8388608.f;
+  static constexpr uint32_t kLowPair = kHalf ? 0xfb53fb53u : 0xcb80cb80u;
 };
 template <typename T>
 __device__ __forceinline__ bool lp_wide(float m) { return !(m > LpRange<T>::kWide && m < LpRange<T>::kHigh); }
+constexpr float kLpLog2e = 1.4426950408889634f, kLpLn2 = 0.6931471805599453f;
+template <typename T>
+__device__ __forceinline__ float lp_rest(float m) {            // m log2(e) less the reference of a range's sums with this maximum
+  return lp_wide<T>(m) ? 0.f : fmaf(m, kLpLog2e, -__fmul_rn(m, kLpLog2e));
+}
 __device__ __forceinline__ float lp_max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -150,7 +157,6 @@ __device__ __forceinline__ uint4 lp_stream(const uint4* p) {
   return r;
 }
 
-constexpr float kLpLog2e = 1.4426950408889634f, kLpLn2 = 0.6931471805599453f;
 constexpr float kLpSlack = 4.f;            // a thread's sums are taken anew when a logit passes their reference by more
 
 constexpr int kLpMaxCluster = 8;
@@ -171,15 +177,23 @@ struct LpStats {
     s += o.s;
     w += o.w;
   }
-  // the same with respect to another part's maximum
-  template <typename T>
-  __device__ __forceinline__ LpStats to(float max) const {
+  __device__ __forceinline__ LpStats at(float max, float t) const {
     LpStats r = *this;
     if (m == max) return r;
-    const float t = lp_wide<T>(m) || lp_wide<T>(max) ? (m - max) * kLpLog2e : __fmul_rn(m, kLpLog2e) - __fmul_rn(max, kLpLog2e);
     r.m = max;
     r.shift(fmaxf(t, -1000.f));
     return r;
+  }
+  // A warp's sums, which refer to a rounded product whatever its maximum, with respect to the maximum of a range that is not wide ...
+  template <typename T>
+  __device__ __forceinline__ LpStats in_range(float max) const {
+    return at(max, __fmul_rn(fmaxf(m, LpRange<T>::kLow), kLpLog2e) - __fmul_rn(max, kLpLog2e));
+  }
+  // ... and a range's with respect to the row's, either of which may be.
+  template <typename T>
+  __device__ __forceinline__ LpStats in_row(float max) const {
+    if (lp_wide<T>(m) || lp_wide<T>(max)) return at(max, (m - max) * kLpLog2e + (lp_rest<T>(max) - lp_rest<T>(m)));
+    return at(max, __fmul_rn(m, kLpLog2e) - __fmul_rn(max, kLpLog2e));
   }
 };
 
@@ -346,17 +360,17 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(con
   float tok_x = logit(tok);
 
   // the CTA's sums: the threads' of each warp with respect to the warp's maximum, then the warps'
-  auto join = [&](const LpStats* part, int parts) {
+  auto join = [&](const LpStats* part, int parts, auto to) {
     float m = part[0].m;
     for (int i = 1; i < parts; ++i) m = fmaxf(m, part[i].m);
     LpStats all = {m, 0.f, 0.f};
-    for (int i = 0; i < parts; ++i) all.add(part[i].to<T>(m));
+    for (int i = 0; i < parts; ++i) all.add(to(part[i], m));
     return all;
   };
   {
     const float2 s = unpack_f32x2(s2), w = unpack_f32x2(w2);
     LpStats st = {warp_max(best), s.x + s.y, w.x + w.y};
-    // (a warp without logits above kLow leaves a sum that `to` takes away; t is not finite only where the row is taken anew)
+    // (a warp without logits above kLow leaves a sum that `in_range` takes away; t is large only where the range is taken anew)
     st.shift(m2 - __fmul_rn(fmaxf(st.m, LpRange<T>::kLow), kLpLog2e));
     st.s = warp_sum(st.s);
     st.w = warp_sum(st.w);
@@ -376,7 +390,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(con
   }
   LpStats mine;
   if (!again) {
-    mine = join(sh.stat, kWarps);
+    mine = join(sh.stat, kWarps, [](const LpStats& s, float max) { return s.in_range<T>(max); });
   } else {
     float m = sh.stat[0].m;
     for (int w = 1; w < kWarps; ++w) m = fmaxf(m, sh.stat[w].m);
@@ -509,7 +523,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(con
     __syncwarp();
     cluster_sync_pair();
     if (rank != 0) return;
-    mine = join(sh.part, cluster);
+    mine = join(sh.part, cluster, [](const LpStats& s, float max) { return s.in_row<T>(max); });
     if constexpr (kTop) {                                      // the CTAs' lists, two by two
       for (int gap = 1; gap < cluster; gap *= 2) {
         const int c = 2 * gap * warp;
@@ -525,7 +539,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(con
   auto logp = [&](float x) {
     if (bad) return nan;
     if (!(x > -INFINITY)) return -INFINITY;
-    if (wide || lp_wide<T>(x)) return (x == mine.m ? 0.f : x - mine.m) - log_s * kLpLn2;
+    if (wide || lp_wide<T>(x)) return (x == mine.m ? 0.f : x - mine.m) - (log_s - lp_rest<T>(mine.m)) * kLpLn2;
     return (fmaf(x, kLpLog2e, -__fmul_rn(mine.m, kLpLog2e)) - log_s) * kLpLn2;
   };
   if (tid == 0) p.entropy[row] = bad ? nan : mine.s > 0.f ? (log_s - mine.w / mine.s) * kLpLn2 : 0.f;

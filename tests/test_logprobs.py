@@ -486,3 +486,54 @@ def test_head_in_chunks_streams_and_graphs(monkeypatch):
     again = ops.linear_logprobs(x[100:109], lw, ids[:9])
     assert torch.equal(p.logprob, again.logprob) and torch.equal(q.logprob, want.logprob) and torch.equal(q.entropy, want.entropy)
     assert ops.device_status(x.device) == 0
+
+
+def far(v, dtype, seed=0):
+    """Rows whose largest logit, or whose masks, lie where a product with log2(e) is rounded by more than an exponential bears: beyond 1e9 on
+    either side, and on both sides of the border (2^23; of fp16 -59000) between the sums' two references, in every part of a row."""
+    g = torch.Generator().manual_seed(seed)
+    noise = torch.randn(v, generator=g) * 2
+    first = torch.arange(v) < v // 2
+    half = torch.finfo(dtype).max < 1e6
+    out = []
+    for top in (6e4, -6e4) if half else (5e9, 1e10, 1e12, 1e20, 1e28, -3e9):
+        z = noise.clone()
+        z[v // 3] = top
+        out += [z, z.flip(0)]
+    for level in (-59000.0, -60000.0, -65504.0) if half else (-3e9, -1e10, -1e11, -1e12, -1e15, 1e10, 1e20):
+        out.append(torch.full((v,), level))
+    for mask in (-59000.0, -6e4) if half else (-1e7, -1.7e9, -2.5e9, -1e10, -1e15):
+        out += [torch.where(first, mask, noise), torch.where(first, noise, mask), torch.where(torch.arange(v) % 64 < 40, mask, noise)]
+    step = 32.0 if half else 1.0                           # (a unit in the last place there)
+    for border in (-59008.0,) if half else (2.0 ** 23, -2.0 ** 23):
+        ladder = border + step * torch.randint(-3, 4, (v,), generator=g)
+        low, high = border - step * (1 + torch.arange(v) % 2), border + step * (1 + torch.arange(v) % 2)
+        out += [ladder, torch.where(first, low, high), torch.where(first, high, low), torch.where(torch.arange(v) == v - 1, high, low),
+                torch.where(torch.arange(v) == 0, high, low)]
+    return torch.stack(out).to(dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("v", [5, 33, 1000, 20011, 131077])
+@pytest.mark.parametrize("top", [0, 6])
+def test_rows_far_from_zero(dtype, v, top):
+    z = far(v, dtype, v)
+    ids = torch.stack([torch.zeros(len(z)), torch.full((len(z),), v - 1), torch.full((len(z),), v // 3), torch.full((len(z),), v // 2)], 1).long()
+    check(z, ids, top, ops.token_logprobs(z.to(DEV), ids.to(DEV), top))
+    for i in range(len(z)):                                # a row by itself: as many CTAs share it as may
+        check(z[i:i + 1], ids[i:i + 1], top, ops.token_logprobs(z[i:i + 1].to(DEV), ids[i:i + 1].to(DEV), top))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,v", [(torch.float32, 32771), (torch.bfloat16, 65543), (torch.float16, 65543)])
+@pytest.mark.parametrize("top", [0, 6])
+def test_many_rows_far_from_zero(dtype, v, top):
+    """In the form for many long rows."""
+    z = far(v, dtype, v)
+    n = len(z)
+    ids = torch.stack([torch.zeros(n), torch.full((n,), v - 1), torch.full((n,), v // 3)], 1).long()
+    times = 2400 // n + 1
+    got = ops.token_logprobs(z.to(DEV).repeat(times, 1), ids.to(DEV).repeat(times, 1), top)
+    for k in (0, times - 1):
+        check(z, ids, top, ops.TokenLogprobs(*(None if f is None else f[n * k:n * (k + 1)] for f in got)))
