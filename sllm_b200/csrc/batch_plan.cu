@@ -160,9 +160,10 @@ SLLM_EXPORT int sllm_batch_plan(const int* new_lens, const int* starts, const in
   const long long units = p.row_units + static_cast<long long>(requests) * p.col_units;
   if (units > INT_MAX) return SLLM_ERR_LIMIT;
   const size_t smem = sizeof(PlanAt) * (requests + 1);
-  // (always the most that a call takes: a smaller figure would refuse the launch of a larger call on another thread)
+  // (always the most that a call takes: a smaller figure would refuse the launch of a larger call on another thread; without it a launch
+  // has 48 KB, the kernel's own array among them)
   constexpr int kMostSmem = static_cast<int>(sizeof(PlanAt)) * (kPlanRequests + 1);
-  if (smem > 48 * 1024 && cudaFuncSetAttribute(batch_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem) != cudaSuccess)
+  if (smem + sizeof(PlanAt) * (kPlanThreads / 32) > 48 * 1024 && cudaFuncSetAttribute(batch_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem) != cudaSuccess)
     return SLLM_ERR_CUDA;
   const int fill = 148 * (smem > 96 * 1024 ? 1 : smem > 48 * 1024 ? 2 : 4);
   const int ctas = static_cast<int>(units < 1 ? 1 : units < fill ? units : fill);

@@ -151,3 +151,30 @@ def test_calls_from_two_threads():
     for t in threads:
         t.join()
     assert not failed, failed
+
+
+AROUND = """
+import sys, torch
+sys.path.insert(0, {root!r})
+from sllm_b200 import ops
+for s in {sizes}:
+    new, starts = torch.arange(s, dtype=torch.int32) % 3, torch.arange(s, dtype=torch.int32) % 7
+    pages = torch.randperm(int(((new + starts + 3) // 4).sum())).to(torch.int32)
+    want = ops.batch_plan(new, starts, pages, int(new.sum()) + 1, 3, 4)
+    got = ops.batch_plan(new.cuda(), starts.cuda(), pages.cuda(), int(new.sum()) + 1, 3, 4)
+    assert all(torch.equal(a, b.cpu()) for a, b in zip(want, got)), s
+print("PLANS_OK")
+"""
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sizes", [[4095, 4096, 6134, 6135], [6136], [6143], [6144], [6137, 6140, 6142, 6145, 16384, 6139, 1]])
+def test_plans_around_the_default_shared_memory(sizes):
+    """Running sums of 6135 requests and the kernel's own 64 bytes are 48 KB; in a process of its own, since a larger plan raises the
+    allowance for what follows."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    proc = subprocess.run([sys.executable, "-c", AROUND.format(root=root, sizes=sizes)], capture_output=True, text=True, timeout=240)
+    assert proc.returncode == 0 and "PLANS_OK" in proc.stdout, proc.stderr[-2000:]
