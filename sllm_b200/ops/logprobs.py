@@ -129,6 +129,29 @@ def _head_floats(n: int, bn: int) -> int:
     return floats
 
 
+def _check_operands(x, w) -> None:
+    """The kernels read rows and weights as bytes of the types and in the order that they expect."""
+    xd = x.data if isinstance(x, core.QTensor) else x
+    if not isinstance(xd, torch.Tensor) or xd.dim() != 2 or xd.shape[1] != w.in_features:
+        raise ValueError("x is [rows, in_features]")
+    stored = w.w4.tiles if w.kind == "w4" else w.w
+    if any(t is not None and t.device != xd.device for t in (stored, w.scale_t, x.scale if isinstance(x, core.QTensor) else None)):
+        raise ValueError("rows and weight are on one device")
+    on_gpu = xd.is_cuda or _lib.fake_active()
+    if isinstance(x, core.QTensor):
+        if w.kind != "fp8" or xd.dtype not in (torch.uint8, torch.float8_e4m3fn) or x.scale.dtype != torch.float32 \
+                or x.scale.shape != ((w.in_features + 127) // 128, xd.shape[0]):
+            raise ValueError("quantised rows are E4M3 with fp32 scales [width / 128, rows], for FP8 weights")
+    elif xd.dtype not in (torch.bfloat16, torch.float32) or (w.kind == "dense" and w.w.dtype not in (torch.bfloat16, torch.float32)):
+        raise ValueError("rows and dense weights are bf16 or fp32")
+    elif on_gpu and xd.dtype != (w.w.dtype if w.kind == "dense" else torch.bfloat16):
+        raise ValueError("on a GPU, rows have a dense weight's type and are bf16 for quantised ones")
+    if on_gpu and w.kind != "w4" and not w.w.is_contiguous():
+        rows_of_any_stride = w.kind == "dense" and (xd.dtype == torch.float32 or w.in_features % 8 != 0) and w.w.stride(1) == 1
+        if not rows_of_any_stride:
+            raise ValueError("the weight is contiguous")
+
+
 def _head(x: torch.Tensor, w: torch.Tensor, tokens: torch.Tensor, softcap: float) -> TokenLogprobs:
     """bf16 rows against a dense matrix on the tensor cores, without logits in memory."""
     r, n, dev = x.shape[0], w.shape[0], x.device
@@ -159,13 +182,11 @@ def _head(x: torch.Tensor, w: torch.Tensor, tokens: torch.Tensor, softcap: float
 
 def linear_logprobs(x, w, tokens: torch.Tensor, softcap: float = 0.0, top: int = 0) -> TokenLogprobs:
     """`token_logprobs` of the logits x W^T (``softcap`` > 0: softcap * tanh(logit / softcap)) for one token per row, in memory that
-    does not grow with rows * vocabulary.  ``x``: hidden rows [R, d] as `ops.linear` takes them for ``w``; ``tokens`` [R].  Logits of
-    dense weights are not rounded on the way (those of FP8 and 4-bit weights are bf16)."""
+    does not grow with rows * vocabulary.  ``x``: hidden rows [R, d] of the weight's type (bf16 or fp32) for a dense
+    ``w``, bf16 or a `QTensor` for FP8, bf16 for 4 bits; ``tokens`` [R].  Logits of dense weights are not rounded on the way (those of
+    FP8 and 4-bit weights are bf16)."""
+    _check_operands(x, w)
     xd = x.data if isinstance(x, core.QTensor) else x
-    if xd.dim() != 2 or xd.shape[1] != w.in_features:
-        raise ValueError("x is [rows, in_features]")
-    if w.kind != "w4" and w.w.device != xd.device:
-        raise ValueError("rows and weight are on one device")
     if softcap != 0.0 and not MIN_CAP <= softcap <= MAX_CAP:
         raise ValueError(f"the soft cap lies between {MIN_CAP} and {MAX_CAP}, or is 0 for none")
     if not 0 <= top <= MAX_TOP:
@@ -176,6 +197,12 @@ def linear_logprobs(x, w, tokens: torch.Tensor, softcap: float = 0.0, top: int =
     if (not top and w.kind == "dense" and not _lib.on_cpu(xd) and xd.dtype == w.w.dtype == torch.bfloat16 and w.in_features % 8 == 0
             and w.w.is_contiguous() and w.w.data_ptr() % 16 == 0):
         return _head(xd, w.w, tokens, softcap)
+    return _through_logits(x, w, tokens, softcap, top)
+
+
+def _through_logits(x, w, tokens: torch.Tensor, softcap: float, top: int) -> TokenLogprobs:
+    """Products of some rows at a time, and the log-probabilities of their logits."""
+    xd = x.data if isinstance(x, core.QTensor) else x
     step = chunk_rows(w.out_features)
     parts = []
     for lo in range(0, xd.shape[0], step):

@@ -537,3 +537,43 @@ def test_many_rows_far_from_zero(dtype, v, top):
     got = ops.token_logprobs(z.to(DEV).repeat(times, 1), ids.to(DEV).repeat(times, 1), top)
     for k in (0, times - 1):
         check(z, ids, top, ops.TokenLogprobs(*(None if f is None else f[n * k:n * (k + 1)] for f in got)))
+
+
+def _w4(w, fmt="nvfp4"):
+    from sllm_b200.ops.w4 import W4Weight
+    return ops.LinearWeight("w4", None, None, W4Weight.quantize(fmt, w))
+
+
+def test_operand_types_of_linear_logprobs():
+    """Types that a kernel would read as others are refused: on the CPU what no product takes, with a stand-in for the library what the
+    kernels take in one type only."""
+    ids = torch.zeros(3, dtype=torch.int64)
+    dense = lambda dt: ops.LinearWeight("dense", torch.zeros((8, 128), dtype=dt))
+    fp8 = ops.LinearWeight.from_dense(torch.randn(8, 128), "fp8")
+    rows_ = lambda dt: torch.zeros((3, 128), dtype=dt)
+    q = ops.quant_fp8(torch.randn(3, 128))
+    never = [(rows_(torch.float16), dense(torch.bfloat16)), (rows_(torch.float16), dense(torch.float16)), (rows_(torch.float32), dense(torch.float16)),
+             (rows_(torch.int32), dense(torch.float32)), (rows_(torch.float64), dense(torch.float64)), (rows_(torch.float16), fp8), (q, dense(torch.bfloat16)),
+             (ops.QTensor(q.data, q.scale[:, :2]), fp8), (ops.QTensor(q.data, q.scale.double()), fp8), (ops.QTensor(q.data.float(), q.scale), fp8),
+             (ops.QTensor(q.data[0], q.scale), fp8), (rows_(torch.float16), _w4(torch.randn(8, 128))), (q, _w4(torch.randn(8, 128))), (None, fp8),
+             (rows_(torch.float32), ops.LinearWeight("fp8", fp8.w, fp8.scale_t.to("meta"))), (rows_(torch.float32).to("meta"), _w4(torch.randn(8, 128)))]
+    on_a_gpu = [(rows_(torch.float32), dense(torch.bfloat16)), (rows_(torch.bfloat16), dense(torch.float32)), (rows_(torch.float32), fp8),
+                (rows_(torch.float32), _w4(torch.randn(8, 128))),
+                (rows_(torch.bfloat16), ops.LinearWeight("dense", torch.zeros((8, 256), dtype=torch.bfloat16)[:, :128])),
+                (rows_(torch.float32), ops.LinearWeight("dense", torch.zeros((128, 8)).t())),
+                (rows_(torch.bfloat16), ops.LinearWeight("fp8", torch.zeros((8, 256), dtype=torch.uint8)[:, :128], fp8.scale_t))]
+    for x, w in on_a_gpu[:4]:
+        ops.linear_logprobs(x, w, ids)                     # (the CPU's oracle takes them as they are)
+    fake = _lib.FakeKernelLibrary()
+    for x, w in never:
+        with pytest.raises(ValueError):
+            ops.linear_logprobs(x, w, ids)
+    _lib.install_fake(fake)
+    try:
+        for x, w in never + on_a_gpu:
+            for top in (0, 2):
+                with pytest.raises(ValueError):
+                    ops.linear_logprobs(x, w, ids, top=top)
+        assert not [c for c in fake.calls if c[0] != "sllm_head_logprobs_floats"]
+    finally:
+        _lib.install_fake(None)
