@@ -152,6 +152,15 @@ def _check_operands(x, w) -> None:
             raise ValueError("the weight is contiguous")
 
 
+def _plain_rows(x: torch.Tensor, strided: bool) -> torch.Tensor:
+    """Rows that a TMA copy can address: whole 16-byte units from a 16-byte boundary on, with ``strided`` any number of them apart."""
+    if not strided or x.stride(1) != 1 or x.stride(0) % 8 or x.stride(0) < x.shape[1]:
+        x = x.contiguous()
+        if x.stride(0) != x.shape[1]:                      # (a single row keeps whichever stride it had)
+            x = x.as_strided(x.shape, (x.shape[1], 1))
+    return x.clone() if x.data_ptr() % 16 else x
+
+
 def _head(x: torch.Tensor, w: torch.Tensor, tokens: torch.Tensor, softcap: float) -> TokenLogprobs:
     """bf16 rows against a dense matrix on the tensor cores, without logits in memory."""
     r, n, dev = x.shape[0], w.shape[0], x.device
@@ -159,8 +168,7 @@ def _head(x: torch.Tensor, w: torch.Tensor, tokens: torch.Tensor, softcap: float
     lp, entropy = out.as_strided((r,), (1,), 0), out.as_strided((r,), (1,), r)
     if not r:
         return TokenLogprobs(lp, entropy)
-    if x.stride(1) != 1 or x.stride(0) % 8 or x.stride(0) < x.shape[1] or x.data_ptr() % 16:      # (a TMA copy needs rows of whole 16 bytes)
-        x = x.contiguous().clone() if x.data_ptr() % 16 else x.contiguous()
+    x = _plain_rows(x, True)
     if tokens.dtype == torch.int64:
         tokens = tokens.clamp(-1, n).to(torch.int32)
     tokens = tokens.contiguous()
@@ -182,7 +190,7 @@ def _head(x: torch.Tensor, w: torch.Tensor, tokens: torch.Tensor, softcap: float
 
 def linear_logprobs(x, w, tokens: torch.Tensor, softcap: float = 0.0, top: int = 0) -> TokenLogprobs:
     """`token_logprobs` of the logits x W^T (``softcap`` > 0: softcap * tanh(logit / softcap)) for one token per row, in memory that
-    does not grow with rows * vocabulary.  ``x``: hidden rows [R, d] of the weight's type (bf16 or fp32) for a dense
+    does not grow with rows * vocabulary.  ``x``: hidden rows [R, d] of any strides, of the weight's type (bf16 or fp32) for a dense
     ``w``, bf16 or a `QTensor` for FP8, bf16 for 4 bits; ``tokens`` [R].  Logits of dense weights are not rounded on the way (those of
     FP8 and 4-bit weights are bf16)."""
     _check_operands(x, w)
@@ -202,7 +210,11 @@ def linear_logprobs(x, w, tokens: torch.Tensor, softcap: float = 0.0, top: int =
 
 def _through_logits(x, w, tokens: torch.Tensor, softcap: float, top: int) -> TokenLogprobs:
     """Products of some rows at a time, and the log-probabilities of their logits."""
-    xd = x.data if isinstance(x, core.QTensor) else x
+    if isinstance(x, core.QTensor):
+        xd = _plain_rows(x.data, False)
+        x = core.QTensor(xd, x.scale)
+    else:
+        xd = x = _plain_rows(x, w.kind == "dense")
     step = chunk_rows(w.out_features)
     parts = []
     for lo in range(0, xd.shape[0], step):

@@ -575,5 +575,31 @@ def test_operand_types_of_linear_logprobs():
                 with pytest.raises(ValueError):
                     ops.linear_logprobs(x, w, ids, top=top)
         assert not [c for c in fake.calls if c[0] != "sllm_head_logprobs_floats"]
+        # rows that the quantiser, which takes no stride, would read from elsewhere
+        wide = torch.zeros((3, 256), dtype=torch.bfloat16)
+        for x in (wide[:, :128], wide[:, ::2], torch.zeros((128, 3), dtype=torch.bfloat16).t(), torch.zeros((3, 129), dtype=torch.bfloat16)[:, 1:]):
+            fake.calls.clear()
+            ops.linear_logprobs(x, fp8, ids)
+            at = [c[1][0] for c in fake.calls if c[0] == "sllm_quant_fp8_1x128"]
+            assert len(at) == 1 and getattr(at[0], "value", at[0]) != x.data_ptr()
     finally:
         _lib.install_fake(None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["dense", "fp32", "fp8", "w4"])
+@pytest.mark.parametrize("top", [0, 3])
+@pytest.mark.parametrize("r", [1, 5, 140])
+def test_rows_of_any_strides_give_the_same(kind, top, r):
+    x, w, ids = head_case(r, 128, 1000, 4)
+    lw = {"dense": lambda: ops.LinearWeight("dense", w), "fp32": lambda: ops.LinearWeight("dense", w.float()),
+          "fp8": lambda: ops.LinearWeight.from_dense(w.cpu().float(), "fp8").to(DEV), "w4": lambda: _w4(w.cpu().float()).to(DEV)}[kind]()
+    x = x.float() if kind == "fp32" else x
+    want = ops.linear_logprobs(x, lw, ids, top=top)
+    new = lambda *shape: torch.full(shape, 9.0, dtype=x.dtype, device=DEV)
+    for view in (new(r, 256)[:, 8:136], new(r, 256)[:, ::2], new(r, 256)[:, 3:131], new(128, r).t(), new(r, 129)[:, 1:], new(r, 1, 128)[:, 0]):
+        view.copy_(x)
+        got = ops.linear_logprobs(view, lw, ids, top=top)
+        assert all(a is None or torch.equal(a, b) for a, b in zip(got, want))
+    one = x[:1].expand(r, -1)
+    assert all(a is None or torch.equal(a, b) for a, b in zip(ops.linear_logprobs(one, lw, ids, top=top), ops.linear_logprobs(one.contiguous(), lw, ids, top=top)))
