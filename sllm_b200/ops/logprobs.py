@@ -205,6 +205,9 @@ def linear_logprobs(x, w, tokens: torch.Tensor, softcap: float = 0.0, top: int =
     if (not top and w.kind == "dense" and not _lib.on_cpu(xd) and xd.dtype == w.w.dtype == torch.bfloat16 and w.in_features % 8 == 0
             and w.w.is_contiguous() and w.w.data_ptr() % 16 == 0):
         return _head(xd, w.w, tokens, softcap)
+    if xd.is_cuda and xd.device.index != torch.cuda.current_device():      # (the products launch on the current device)
+        with torch.cuda.device(xd.device):
+            return _through_logits(x, w, tokens, softcap, top)
     return _through_logits(x, w, tokens, softcap, top)
 
 

@@ -603,3 +603,29 @@ def test_rows_of_any_strides_give_the_same(kind, top, r):
         assert all(a is None or torch.equal(a, b) for a, b in zip(got, want))
     one = x[:1].expand(r, -1)
     assert all(a is None or torch.equal(a, b) for a, b in zip(ops.linear_logprobs(one, lw, ids, top=top), ops.linear_logprobs(one.contiguous(), lw, ids, top=top)))
+
+
+def test_products_run_on_the_device_of_their_rows(monkeypatch):
+    """A device that is not current stood in for: it is current while the logits are made."""
+    now, seen = [0], []
+
+    class On:
+        def __init__(self, device):
+            self.index = device.index
+
+        def __enter__(self):
+            self.before, now[0] = now[0], self.index
+
+        def __exit__(self, *exc):
+            now[0] = self.before
+
+    class Rows:
+        is_cuda, dtype, device, shape = True, torch.float32, torch.device("cuda", 1), (3, 8)
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: now[0])
+    monkeypatch.setattr(torch.cuda, "device", On)
+    monkeypatch.setattr(LP, "_check_operands", lambda x, w: None)
+    monkeypatch.setattr(LP, "_check_tokens", lambda *a: None)
+    monkeypatch.setattr(LP, "_through_logits", lambda *a: seen.append(now[0]))
+    ops.linear_logprobs(Rows(), ops.LinearWeight("dense", torch.zeros(5, 8)), torch.zeros(3, dtype=torch.int64), top=1)
+    assert seen == [1] and now == [0]
