@@ -35,6 +35,10 @@ class StateSlots:
             t.select(dim, s).zero_()
         return s
 
+    @property
+    def free_slots(self) -> int:
+        return len(self._free)
+
     def free_slot(self, seq_id: int) -> None:
         s = self.slot_of.pop(seq_id, None)
         if s is not None:

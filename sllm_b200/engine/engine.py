@@ -233,17 +233,22 @@ class Engine:
     def score(self, prompts: list, top: int = 0, max_rows: int = SCORE_ROWS) -> list:
         """What the model makes of given texts: per token list a `TokenLogprobs` on the CPU whose row i belongs to token i + 1 - its
         log-probability after the tokens ahead of it, the entropy of that distribution and (with ``top``) its likeliest tokens.
-        Texts run together up to ``max_rows`` tokens, a longer one in portions, on scratch pages that are released again.  Without
+        Texts run together up to ``max_rows`` tokens and as many as the free pages and recurrent-state slots hold, a longer one in
+        portions, on scratch pages that are released again; where one alone finds no room, none is run.  Without
         ``top`` a dense output matrix on one GPU yields them without logits in memory, from unrounded sums; other heads go through
         logits as `forward` gives them."""
         self._guard()
         prompts = [list(p) for p in prompts]
         self.check_score(prompts, top, max_rows)
+        self._check_score_room(prompts)
         out, i = [], 0
         while i < len(prompts):
-            j, rows = i + 1, len(prompts[i])
-            while j < len(prompts) and j - i < self.max_batch and rows + len(prompts[j]) <= max_rows:
+            free, most = self.cache.pool.stats()["free"], min(self.max_batch, self.cache.free_slots) if self.has_state else self.max_batch
+            j, rows, pages = i + 1, len(prompts[i]), self._pages_of(prompts[i])
+            while (j < len(prompts) and j - i < most and rows + len(prompts[j]) <= max_rows
+                   and pages + self._pages_of(prompts[j]) <= free):
                 rows += len(prompts[j])
+                pages += self._pages_of(prompts[j])
                 j += 1
             out += self._score_together(prompts[i:j], top, max_rows)
             i = j
@@ -255,6 +260,16 @@ class Engine:
             raise ValueError("a scored text has between one token and the context's length, all inside the vocabulary")
         if not 0 <= top <= ops.logprobs.MAX_TOP or max_rows < 1:
             raise ValueError(f"top lies between 0 and {ops.logprobs.MAX_TOP}, max_rows at 1 or more")
+
+    def _pages_of(self, tokens: list) -> int:
+        return -(-len(tokens) // self.cfg.page_size)
+
+    def _check_score_room(self, prompts: list) -> None:
+        free = self.cache.pool.stats()["free"]
+        if any(self._pages_of(p) > free for p in prompts):
+            raise OutOfPages(f"no free KV pages for {max(map(len, prompts))} tokens")
+        if prompts and self.has_state and not self.cache.free_slots:
+            raise RuntimeError("no free recurrent-state slot")
 
     def _score_together(self, prompts: list, top: int, max_rows: int) -> list:
         pool, seqs, found = self.cache.pool, [], [[] for _ in prompts]

@@ -103,6 +103,46 @@ def test_score_refusals_leave_nothing_behind():
     assert st["sequences"] == 0 and st["free"] == st["pages"]
 
 
+def test_score_runs_as_many_texts_as_there_is_room_for(monkeypatch):
+    """Texts that fit alone but not together, beside a live sequence; in groups that fill the pages."""
+    eng = build_engine(MC.tiny_llama(), "cpu", num_pages=9, max_batch=4)
+    texts = [[3 + (7 * i + k) % 50 for k in range(n)] for i, n in enumerate((60, 50, 64, 1, 33, 64, 2, 16))]
+    want = [build_engine(MC.tiny_llama(), "cpu", num_pages=9, max_batch=4).score([t], 2)[0] for t in texts]
+    live = eng.new_sequence([1, 2, 3])
+    eng.prefill([live])
+    groups = []
+    run = eng._score_together
+    monkeypatch.setattr(eng, "_score_together", lambda prompts, *a: groups.append([len(p) for p in prompts]) or run(prompts, *a))
+    got = eng.score(texts, 2)
+    assert groups == [[60, 50], [64, 1, 33], [64, 2, 16]]
+    for a, b in zip(got, want):
+        assert torch.equal(a.top_ids, b.top_ids) and torch.allclose(a.logprob, b.logprob, atol=1e-4) and torch.allclose(a.entropy, b.entropy, atol=1e-4)
+    from sllm_b200.cache.paged import OutOfPages
+    groups.clear()
+    with pytest.raises(OutOfPages):
+        eng.score([[1, 2], [3] * 129])
+    assert groups == []                                    # refused ahead of any work
+    st = eng.cache.pool.stats()
+    assert st["sequences"] == 1 and st["free"] == 8
+
+
+def test_score_runs_as_many_texts_as_there_are_state_slots():
+    from sllm_b200.models.qwen35 import tiny_qwen35
+    make = lambda: build_engine(tiny_qwen35(), "cpu", num_pages=32, max_batch=2)
+    eng, texts = make(), [[5, 9, 3], [11, 4], [8, 8, 8, 1]]
+    want = [make().score([t])[0] for t in texts]
+    live = [eng.new_sequence([1]) for _ in range(eng.cache.free_slots - 1)]
+    for a, b in zip(eng.score(texts), want):
+        assert torch.allclose(a.logprob, b.logprob, atol=1e-4)
+    assert eng.cache.free_slots == 1
+    last = eng.new_sequence([1])
+    with pytest.raises(RuntimeError, match="slot"):
+        eng.score(texts)
+    assert eng.score([]) == [] and eng.cache.pool.stats()["sequences"] == len(live) + 1
+    eng.free_sequence(last)
+    assert len(eng.score(texts)) == 3
+
+
 def test_page_lists():
     eng = build_engine(MC.tiny_llama(), "cpu", num_pages=16, max_batch=2)
     pool = eng.cache.pool
