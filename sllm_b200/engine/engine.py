@@ -237,10 +237,8 @@ class Engine:
         portions, on scratch pages that are released again; where one alone finds no room, none is run.  Without
         ``top`` a dense output matrix on one GPU yields them without logits in memory, from unrounded sums; other heads go through
         logits as `forward` gives them."""
-        self._guard()
         prompts = [list(p) for p in prompts]
         self.check_score(prompts, top, max_rows)
-        self._check_score_room(prompts)
         out, i = [], 0
         while i < len(prompts):
             free, most = self.cache.pool.stats()["free"], min(self.max_batch, self.cache.free_slots) if self.has_state else self.max_batch
@@ -255,21 +253,20 @@ class Engine:
         return out
 
     def check_score(self, prompts: list, top: int, max_rows: int) -> None:
-        """Raises for arguments that `score` refuses."""
+        """Raises for arguments that `score` refuses and where it finds no room."""
+        self._guard()
         if any(not 1 <= len(p) <= self.cfg.max_context or min(p) < 0 or max(p) >= self.cfg.vocab for p in prompts):
             raise ValueError("a scored text has between one token and the context's length, all inside the vocabulary")
         if not 0 <= top <= ops.logprobs.MAX_TOP or max_rows < 1:
             raise ValueError(f"top lies between 0 and {ops.logprobs.MAX_TOP}, max_rows at 1 or more")
-
-    def _pages_of(self, tokens: list) -> int:
-        return -(-len(tokens) // self.cfg.page_size)
-
-    def _check_score_room(self, prompts: list) -> None:
         free = self.cache.pool.stats()["free"]
         if any(self._pages_of(p) > free for p in prompts):
             raise OutOfPages(f"no free KV pages for {max(map(len, prompts))} tokens")
         if prompts and self.has_state and not self.cache.free_slots:
             raise RuntimeError("no free recurrent-state slot")
+
+    def _pages_of(self, tokens: list) -> int:
+        return -(-len(tokens) // self.cfg.page_size)
 
     def _score_together(self, prompts: list, top: int, max_rows: int) -> list:
         pool, seqs, found = self.cache.pool, [], [[] for _ in prompts]
