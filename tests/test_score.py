@@ -198,6 +198,13 @@ def test_score_without_room_leaves_the_followers_serving():
     assert proc.returncode == 0 and "SCORE_ROOM_OK" in proc.stdout, proc.stdout[-2000:] + proc.stderr[-3000:]
 
 
+def test_score_of_a_head_sharded_over_ranks():
+    worker = os.path.join(os.path.dirname(os.path.abspath(__file__)), "score_tp_worker.py")
+    proc = subprocess.run([sys.executable, "-m", "torch.distributed.run", "--nnodes=1", "--nproc-per-node=2", "--master-addr", "127.0.0.1",
+                           "--master-port", "29851", worker], capture_output=True, text=True, timeout=240)
+    assert proc.returncode == 0 and "SCORE_TP_OK" in proc.stdout, proc.stdout[-2000:] + proc.stderr[-3000:]
+
+
 # ------------------------------------------------------------------------------------------ GPU
 @pytest.mark.gpu
 def test_prefill_batches_are_the_same_on_the_gpu():
