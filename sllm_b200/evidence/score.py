@@ -4,7 +4,8 @@
 
 Prints one JSON line (schema ``sllm-score-v1``): per text its tokens, the log-probability of every token after the first, the
 entropy of the distribution it was taken from, the mean negative log-likelihood and the perplexity (null for a text of one
-token), and with ``--top`` the likeliest tokens of every place.  Exit codes as the command line's (2 usage, 3 model file, 4 device).
+token), and with ``--top`` the likeliest tokens of every place.  Numbers that are not finite (a token that is shut out, logits
+that are NaN) are null.  Exit codes as the command line's (2 usage, 3 model file, 4 device).
 """
 from __future__ import annotations
 
@@ -16,16 +17,20 @@ from ..cli.common import CliError, StrictParser, add_model_source, emit, open_mo
 SCHEMA = "sllm-score-v1"
 
 
+def _finite(x):
+    return [_finite(v) for v in x] if isinstance(x, list) else x if x is not None and math.isfinite(x) else None
+
+
 def score_texts(eng, token_lists: list, top: int = 0) -> list:
     """One record per token list, from `Engine.score`."""
     out = []
     for ids, lp in zip(token_lists, eng.score(token_lists, top)):
         n = lp.logprob.numel()
         nll = -float(lp.logprob.double().sum()) / n if n else None
-        rec = {"tokens": list(ids), "logprobs": lp.logprob.tolist(), "entropy": lp.entropy.tolist(), "nll_mean": nll,
+        rec = {"tokens": list(ids), "logprobs": _finite(lp.logprob.tolist()), "entropy": _finite(lp.entropy.tolist()), "nll_mean": _finite(nll),
                "perplexity": math.exp(nll) if n and nll < 700 else None}
         if top:
-            rec["top"] = [[{"token": t, "logprob": p} for t, p in zip(ts, ps) if t >= 0]
+            rec["top"] = [[{"token": t, "logprob": _finite(p)} for t, p in zip(ts, ps) if t >= 0]
                           for ts, ps in zip(lp.top_ids.tolist(), lp.top_logprobs.tolist())]
         out.append(rec)
     return out

@@ -184,6 +184,28 @@ def test_score_runner(tmp_path, capsys):
     assert score.main(["--gguf", g, "--derived-lock", str(tmp_path / "none"), "--cpu", "--text", "a"]) == 3
 
 
+def test_score_records_are_json():
+    """What no JSON number stands for - a token that is shut out, a row of NaN, a likelihood beyond the perplexity's range - is null."""
+    from sllm_b200.evidence.score import score_texts
+    inf, nan = float("inf"), float("nan")
+
+    class Stub:
+        def score(self, texts, top):
+            t = torch.tensor
+            return [ops.TokenLogprobs(t([-1.0, -inf]), t([0.5, 0.0]), t([[3, -1], [-1, -1]]), t([[-0.25, -inf], [-inf, -inf]])),
+                    ops.TokenLogprobs(t([nan, -2.0]), t([nan, 1.0]), t([[-1, -1], [4, 2]]), t([[nan, nan], [-0.5, -inf]])),
+                    ops.TokenLogprobs(t([-800.0]), t([0.0]), t([[1, 2]]), t([[0.0, -3.0]])),
+                    ops.TokenLogprobs(torch.empty(0), torch.empty(0), torch.empty((0, 2), dtype=torch.int32), torch.empty((0, 2)))]
+
+    got = json.loads(json.dumps(score_texts(Stub(), [[1, 2, 3], [4, 5, 6], [7, 8], [9]], 2), allow_nan=False))
+    assert got[0]["logprobs"] == [-1.0, None] and got[0]["nll_mean"] is None and got[0]["perplexity"] is None
+    assert got[0]["top"] == [[{"token": 3, "logprob": -0.25}], []]
+    assert got[1]["logprobs"] == [None, -2.0] and got[1]["entropy"] == [None, 1.0] and got[1]["nll_mean"] is None and got[1]["perplexity"] is None
+    assert got[1]["top"][1] == [{"token": 4, "logprob": -0.5}, {"token": 2, "logprob": None}]
+    assert got[2]["nll_mean"] == 800.0 and got[2]["perplexity"] is None
+    assert got[3]["logprobs"] == [] and got[3]["nll_mean"] is None and got[3]["perplexity"] is None
+
+
 def test_score_is_mirrored_to_follower_ranks():
     worker = os.path.join(os.path.dirname(os.path.abspath(__file__)), "score_worker.py")
     proc = subprocess.run([sys.executable, "-m", "torch.distributed.run", "--nnodes=1", "--nproc-per-node=2", "--master-addr", "127.0.0.1",
