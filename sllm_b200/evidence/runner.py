@@ -244,11 +244,11 @@ def _linear_logprobs(size):
         p = ops.linear_logprobs(x, lw, ids)
         return torch.stack([p.logprob, p.entropy])
 
-    z = x.double() @ w.double().t() if size != "large" else None
-    want = None
-    if z is not None:
-        logp = torch.log_softmax(z, 1)
-        want = torch.stack([logp.gather(1, ids.long()[:, None])[:, 0], -(logp.exp() * logp).sum(1)])
+    wd, parts = w.double(), []
+    for lo in range(0, m, 256):                            # (64-bit logits of 256 rows: 0.26 GB at the most)
+        logp = torch.log_softmax(x[lo:lo + 256].double() @ wd.t(), 1)
+        parts.append(torch.stack([logp.gather(1, ids[lo:lo + 256].long()[:, None])[:, 0], -(logp.exp() * logp).sum(1)]))
+    want = torch.cat(parts, 1)
     return run, want, 2 * k * (m + n), 2 * m * n * k, {"m": m, "n": n, "k": k}, (1e-5, 1e-5)
 
 

@@ -95,6 +95,16 @@ def test_roundtrip_on_the_gpu(tmp_path):
     assert set(r["checks"]) == {"gemm_bf16", "gemm_fp8", "rmsnorm", "gated_act", "argmax", "paged_attention"}
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("size,kernel", [("small", "head_few_kernel"), ("large", "head_logprobs_kernel")])
+def test_both_head_kernels_are_checked(size, kernel):
+    """The kernel for few rows and the one on CTA pairs each ran and met 64 bits."""
+    from sllm_b200.evidence.runner import run_op
+    rep = run_op("linear-logprobs", size)
+    assert rep["correctness"]["passed"] and "skipped" not in rep["correctness"], rep["correctness"]
+    assert [d for d in rep["dispatch"] if kernel in json.dumps(d)], rep["dispatch"]
+
+
 def test_accuracy_runner_orders_the_formats_on_the_cpu():
     """KL(bf16 || candidate) over shared seeded weights: identical configurations give zero, FP8 moves the distribution
     less than 4-bit weights, and 4-bit activations add to the 4-bit weights' divergence."""
