@@ -234,9 +234,9 @@ class Engine:
         """What the model makes of given texts: per token list a `TokenLogprobs` on the CPU whose row i belongs to token i + 1 - its
         log-probability after the tokens ahead of it, the entropy of that distribution and (with ``top``) its likeliest tokens.
         Texts run together up to ``max_rows`` tokens and as many as the free pages and recurrent-state slots hold, a longer one in
-        portions, on scratch pages that are released again; where one alone finds no room, none is run.  Without
-        ``top`` a dense output matrix on one GPU yields them without logits in memory, from unrounded sums; other heads go through
-        logits as `forward` gives them."""
+        portions, on scratch pages that are released again; where one alone finds no room, none is run.  A dense
+        output matrix on one GPU yields them from unrounded sums, the same with and without ``top`` (without: no logits in memory); other
+        heads go through logits as `forward` gives them."""
         prompts = [list(p) for p in prompts]
         self.check_score(prompts, top, max_rows)
         out, i = [], 0
@@ -307,13 +307,13 @@ class Engine:
     def _row_logprobs(self, b: ForwardBatch, h: torch.Tensor, rows: torch.Tensor, tokens: torch.Tensor, top: int):
         """`ops.TokenLogprobs` of ``tokens`` after the rows ``rows`` of the residual ``h``."""
         m, cfg = self.model, self.cfg
-        if not top and m.tp.size == 1 and m.w.lm_head.kind == "dense":
+        if m.tp.size == 1 and m.w.lm_head.kind == "dense":
             if hasattr(m, "final_hidden"):
                 x = m.final_hidden(h, rows)
             else:
                 x = ops.rmsnorm(h.index_select(0, rows), m.w.final_norm, cfg.rms_eps, cfg.norm_offset_one)
             capped = cfg.family in ("llama", "gemma4", "sepedra")          # families whose logits pass the soft cap
-            return ops.linear_logprobs(x, m.w.lm_head, tokens, softcap=cfg.logit_softcap if capped else 0.0)
+            return ops.linear_logprobs(x, m.w.lm_head, tokens, softcap=cfg.logit_softcap if capped else 0.0, top=top)
         parts, step = [], ops.logprobs.chunk_rows(cfg.vocab)
         for lo in range(0, rows.numel(), step):
             b.logit_rows = rows[lo:lo + step]

@@ -271,6 +271,24 @@ def test_score_of_every_family():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("which", [0, 1])
+def test_alternatives_do_not_change_a_tokens_score(which):
+    """Both ways sum the products in 32 bits: with a row's largest sum of magnitudes (at most the product of the norms), every 16 of d products
+    are rounded once towards zero, on either way, and the joint sums as in the ops' own tests."""
+    cfg = _families()[which]
+    eng = build_engine(cfg, DEV, seed=1, num_pages=64, max_batch=4)
+    m = eng.model.w
+    mag = float(m.lm_head.w.double().norm(dim=1).max() * (m.final_norm.double().abs().max() + cfg.norm_offset_one) * cfg.d_model ** 0.5)
+    dz, rel = mag * (cfg.d_model / 16 + 8) * 2 ** -23, (cfg.vocab / 256 + 64) * 2 ** -24
+    texts = TEXTS + [[(7 * k) % 900 for k in range(200)]]
+    for a, b in zip(eng.score(texts, 0), eng.score(texts, 3)):
+        if not a.logprob.numel():
+            continue
+        assert float((a.logprob - b.logprob).abs().max()) <= 4 * dz + 2 * rel + 16 * 2 ** -24 * (float(a.logprob.abs().max()) + cfg.logit_softcap)
+        assert float((a.entropy - b.entropy).abs().max()) <= 4 * (dz + rel) * (1 + 2 * mag + float(a.entropy.max()))
+
+
+@pytest.mark.gpu
 def test_wide_tables_decode_the_same():
     eng = build_engine(_bf16(max_context=4096), DEV, seed=1, num_pages=200, max_batch=8)
     prompts = [list(range(3, 40)), [5, 6, 7, 8], [9] * 15]
