@@ -629,3 +629,23 @@ def test_products_run_on_the_device_of_their_rows(monkeypatch):
     monkeypatch.setattr(LP, "_through_logits", lambda *a: seen.append(now[0]))
     ops.linear_logprobs(Rows(), ops.LinearWeight("dense", torch.zeros(5, 8)), torch.zeros(3, dtype=torch.int64), top=1)
     assert seen == [1] and now == [0]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("r", [8, 200])
+def test_head_sums_leave_the_tensor_core_every_512_columns(r):
+    """One product of 1 and 4095 of 2^-26, which next to it a tensor core's sum loses: those of its chain of 512 columns, 511 of them, while
+    the others reach the token's logit whole.  A chain of 1024 loses 1023, 1.4e-5 of the log-probability (the token has 0.07 of the row).
+    Beside the loss: 8 chains added to about 1; 40 terms of the row's sum, added in pairs by a thread and joined (20 + 8 roundings, an
+    exponential's 2^-22), and 8 roundings of numbers of the result's size."""
+    d, v = 4096, 40
+    w = torch.zeros((v, d))
+    w[0] = 2.0 ** -26
+    w[0, 0] = 1.0
+    x, w = torch.ones((r, d), dtype=torch.bfloat16, device=DEV), w.bfloat16().to(DEV)
+    ids = torch.zeros(r, dtype=torch.int32, device=DEV)
+    got = ops.linear_logprobs(x, ops.LinearWeight("dense", w), ids)
+    lp = torch.log_softmax(x.double() @ w.double().t(), 1)[:, 0].cpu()
+    tol = 511 * 2.0 ** -26 + (8 + 20 + 8 + 4) * EPS + 8 * EPS * float(lp.abs().max())
+    assert tol < 1023 * 2.0 ** -26 * (1 - math.exp(float(lp.max()))) - 2e-6
+    same(got.logprob, lp, tol)
