@@ -168,7 +168,7 @@ class Engine:
 
         cache = self.cache
         staging = sum(nbytes(getattr(self, n)) for n in ("d_tokens", "d_positions", "d_kv_lens", "d_seq_index", "d_table", "d_out",
-                                                        "d_slots", "d_row_off", "d_rope_delta", "d_rope3", "d_logits"))
+                                                        "d_one", "d_slots", "d_row_off", "d_rope_delta", "d_rope3", "d_logits"))
         pinned = sum(nbytes(getattr(self, n)) for n in ("h_tokens", "h_positions", "h_table", "h_out", "h_slots", "h_rope_delta"))
         out = {"weights": weight_bytes(self.model.w, set()),
                "kv_pages": nbytes(getattr(cache, "values", None)), "kv_scales": nbytes(getattr(cache, "scales", None)),

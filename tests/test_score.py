@@ -143,6 +143,12 @@ def test_score_runs_as_many_texts_as_there_are_state_slots():
     assert len(eng.score(texts)) == 3
 
 
+def test_accounting_counts_every_static_input():
+    eng = build_engine(MC.tiny_llama(), "cpu", num_pages=8, max_batch=2)
+    held = sum(t.numel() * t.element_size() for n, t in vars(eng).items() if n.startswith("d_") and isinstance(t, torch.Tensor))
+    assert eng.accounting()["device_staging"] == held
+
+
 def test_page_lists():
     eng = build_engine(MC.tiny_llama(), "cpu", num_pages=16, max_batch=2)
     pool = eng.cache.pool
