@@ -321,6 +321,7 @@ class Engine:
             if z.shape[1] != cfg.vocab:
                 z = m.tp.gather_logits(z)
             parts.append(ops.token_logprobs(z, tokens[lo:lo + step], top))
+            del z                                          # (ahead of the next rows' logits)
         return ops.TokenLogprobs(*(None if f[0] is None else torch.cat(f) for f in zip(*parts)))
 
     def shutdown_report(self) -> dict:

@@ -192,7 +192,8 @@ def linear_logprobs(x, w, tokens: torch.Tensor, softcap: float = 0.0, top: int =
     """`token_logprobs` of the logits x W^T (``softcap`` > 0: softcap * tanh(logit / softcap)) for one token per row, in memory that
     does not grow with rows * vocabulary.  ``x``: hidden rows [R, d] of any strides, of the weight's type (bf16 or fp32) for a dense
     ``w``, bf16 or a `QTensor` for FP8, bf16 for 4 bits; ``tokens`` [R].  Logits of dense weights are not rounded on the way (those of
-    FP8 and 4-bit weights are bf16)."""
+    FP8 and 4-bit weights are bf16).  All but bf16 heads without alternatives go through `ops.linear`, whose workspace serves one
+    stream at a time."""
     _check_operands(x, w)
     xd = x.data if isinstance(x, core.QTensor) else x
     if softcap != 0.0 and not MIN_CAP <= softcap <= MAX_CAP:
@@ -233,6 +234,7 @@ def _through_logits(x, w, tokens: torch.Tensor, softcap: float, top: int) -> Tok
             if softcap:
                 z = core.elementwise("tanh_softcap", z, s=softcap)
         parts.append(token_logprobs(z, tokens[lo:hi], top))
+        del z                                              # (ahead of the next rows' logits)
     if not parts:
         z = torch.empty((0, w.out_features), dtype=torch.float32, device=xd.device)
         return token_logprobs(z, tokens, top)

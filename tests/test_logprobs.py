@@ -131,6 +131,38 @@ def test_linear_in_chunks_gives_the_same(monkeypatch):
     assert none.logprob.shape == (0,) and none.top_ids.shape == (0, 2)
 
 
+def test_logits_of_one_chunk_are_held_at_a_time(monkeypatch):
+    """The chunk's size bounds the memory only if a chunk is gone before the next one is made."""
+    import weakref
+    from sllm_b200.engine.engine import build_engine
+    from sllm_b200.models import config as MC
+    from sllm_b200.ops import core
+    held = []
+    monkeypatch.setattr(LP, "CHUNK_LOGITS", 160)
+
+    def watched(make):
+        def call(*a, **kw):
+            assert not any(r() is not None for r in held)
+            z = make(*a, **kw)
+            held.append(weakref.ref(z))
+            return z
+        return call
+
+    monkeypatch.setattr(core, "linear", watched(core.linear))
+    x, w = torch.randn(11, 16), ops.LinearWeight("dense", torch.randn(40, 16))
+    ops.linear_logprobs(x, w, torch.zeros(11, dtype=torch.int64), top=2)
+    assert len(held) == 3
+    monkeypatch.undo()
+    held.clear()
+    eng = build_engine(MC.tiny_llama(), "cpu", num_pages=8, max_batch=2)
+    monkeypatch.setattr(LP, "CHUNK_LOGITS", 4 * eng.cfg.vocab)
+    monkeypatch.setattr(eng.model.w.lm_head, "kind", "fp8x")                # (a head that goes through the model's logits)
+    head = torch.zeros((eng.cfg.vocab, eng.cfg.d_model))
+    monkeypatch.setattr(eng.model, "logits", watched(lambda h, b: h.index_select(0, b.logit_rows).float() @ head.t()))
+    got = eng.score([[1, 2, 3, 4, 5, 6, 7, 8, 9, 10]], 2)[0]
+    assert len(held) == 3 and got.logprob.shape == (9,)
+
+
 def test_refusals():
     z, ids = torch.zeros(3, 8), torch.zeros(3, dtype=torch.int64)
     w = ops.LinearWeight("dense", torch.zeros(8, 4))
