@@ -9,9 +9,11 @@
 //               count on the first CTA's barrier
 //   warp 1      owns the tensor memory; in the first CTA it issues the products for both
 //   warps 4 ..  two groups of four, thread = row, a group per half of the tile's columns
-// Measured (B200, one launch and the join, m x n x k, us, in brackets what the rates of a copy and of a library product give):
-//      1 x 128256 x 4096     171 (163)         777 x 151936 x 2560, cap    505 (361: 777 rows fill 3.04 tiles)
-//     48 x 201088 x 2880     190 (179)        4096 x 128256 x 4096        2649 (2571)
+// Measured (B200, one launch and the join, m x n x k, us, in brackets what the rates of a copy and of a library product give; calls a
+// few at a time, and behind the stroke one after another for seconds, where the power limit holds the clock at 1.1 to 1.3 GHz):
+//      1 x 128256 x 4096     171 / 184 (163)         777 x 151936 x 2560, cap    536 / 628 (361: 777 rows fill 3.04 tiles)
+//     48 x 201088 x 2880     186 / 206 (179)        4096 x 128256 x 4096        2784 / 3117 (2571; 3119 at the sustained rate)
+// The tensor pipe is busy for 0.89 of the third's cycles (0.98 without the cap), the DRAM at 0.78 of its peak in the first two.
 // The first two through the kernel for few rows; on CTA pairs, whose second half has no rows there, they took 270 and 260.
 // A tile's sum over K is taken in chains of kHlChain K blocks with an accumulator of their own, which the epilogue warps add in fp32
 // registers while the next chain is multiplied: tensor memory rounds towards zero, and a chain's error grows with its length (4096 wide:

@@ -222,11 +222,13 @@ struct __align__(16) LpShared {
 // Alternatives: the top-th largest of the threads' maxima bounds the wanted ones from below, and hardly more parts of threads' units have
 // logits at or above it than there are alternatives; those units are read again (out of L2) and what passes the bound is ranked by
 // counting.  Where more than kLpPool logits pass it (runs of equal or ordered ones), sorted lists are merged 32 at a time instead.
-// What bounds it: memory and the exponentials together for many rows (4096 x 128256 bf16: 172 us of 162.5 at the copy bandwidth, 0.69 of the
-// issue slots; 1500 x 32768 fp16: 23.2 of 15.2, rows start and end too often), for few the chain of a row (one of 128256: 3.9 us, 6.9 with 20
-// alternatives, of which the launch takes 2).
+// What bounds it: memory and the exponentials together for many rows (4096 x 128256 bf16, 162.5 us at the copy bandwidth: 171 to 187 from one
+// process to the next, 178 under the profiler with 0.72 of the DRAM's peak, 0.74 of the exponential unit and 0.62 of the issue slots busy;
+// 1500 x 32768 fp16: 23.2 of 15.2, rows start and end too often), for few the chain of a row (one of 128256: 3.7 us, 7.0 with 20 alternatives,
+// of which the launch takes 2).
 // kLong, for many long rows: rounds of loads without a bound, and the maxima of kLpParts parts of a thread's units, so that less is read
-// again (4096 x 128256 bf16, us: without alternatives 190 -> 184, 5 of them 214 -> 207, 32 of them 316 -> 257; with 700 rows 5 take 43.5 -> 45.3).
+// again (4096 x 128256 bf16, us, both forms in one process: without alternatives 190 -> 184, 5 of them 214 -> 207, 32 of them 316 -> 257;
+// with 700 rows 5 take 43.5 -> 45.3).
 template <typename T, int kThreads, bool kTop, bool kLong>
 __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(const LogprobParams p, int cluster) {
   constexpr int kN = LpVec<T>::kN, kWarps = kThreads / 32, kAhead = 4, kParts = kLong ? kLpParts : 1;
@@ -568,8 +570,9 @@ static cudaError_t logprobs_go(const LogprobParams& p, int cluster, cudaStream_t
 // with CTAs of 64, 128 and 256 threads: 8.5 / 9.7 / 13.3, 13.7 / 12.5 / 18.3, 45.5 / 40.1 / 42.6); longer rows take 128 threads only where the last wave
 // of CTAs is filled as well as with 256 (700 x 50000: 25.3 and 20.0; 1500 x 32768: 24.3 and 23.4).  Few rows do not (138 x 2067 fp32 with 32
 // alternatives: 9.5 with 64 threads, 6.9 with 256): a cluster shares a row, as many CTAs as the card holds at a time and no more (with 5 alternatives
-// bf16: 80 x 128256 13.7 in clusters of eight with 128 threads, 16.5 with 256, which do not fit; 160 x 128256 17.0 in threes, 20.2 in fours; 300 x 32000
-// 11.7 alone, 15.4 in twos; one row 7 in a cluster of eight).
+// bf16: 80 x 128256 13.7 in clusters of eight with 128 threads, 16.5 with 256, which do not fit; 160 x 128256 17.0 in threes, 20.2 in fours; one row
+// 7 in a cluster of eight).  Half of the places and more, in twos or alone: 300 x 32000 15.4 / 11.6, 592 x 128256 37.4 / 32.0, 500 x 128256 34.1 / 31.7;
+// only 300 to 400 rows beyond 100000 logits lose by the rule (300 x 128256 27.7 / 30.5, without alternatives 22.8 / 27.5; 400 x 128256 30.1 / 31.2).
 template <typename T>
 static cudaError_t logprobs_go(const LogprobParams& p, cudaStream_t st) {
   const long long units = (static_cast<long long>(p.vocab) + LpVec<T>::kN - 1) / LpVec<T>::kN;
